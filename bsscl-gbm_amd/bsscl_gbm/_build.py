@@ -21,7 +21,8 @@ LIB_NAME = "libbsscl_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 OBJ_DIR = os.path.join(ROOT, "_build")
 
-SOURCES = ["kernels.hip", "walk.hip", "fisher_yates.hip", "colsort.hip", "engine.hip", "sampler.cpp"]
+SOURCES = ["kernels.hip", "walk.hip", "fisher_yates.hip", "colsort.hip", "engine.hip", "sampler.cpp",
+           "softmax_head.hip", "grad_norm.hip"]
 ARCH = "gfx950"
 
 

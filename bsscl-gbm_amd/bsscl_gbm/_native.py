@@ -80,6 +80,14 @@ _SIGS = {
     "bsscl_engine_set_profiling": [_P, _i32],
     "bsscl_boost_set_pipeline": [_P, _i32],
     "bsscl_engine_stats": [_P, _P, _i32, _P],
+    "bsscl_head_workspace": [_i32, _i64, _i64, _i64, _P, _i64, _i32, _P],
+    "bsscl_head_loss": [_i32, _P, _i32, _P, _i64, _P, _i64, _P, _P, _i64, _i64, _i64, _i32, _f64,
+                        _f64, _P, _P, _P, _P, _i64],
+    "bsscl_head_grad": [_i32, _P, _i32, _P, _i64, _P, _i64, _P, _P, _i64, _i64, _i64, _i32, _f64,
+                        _f64, _f64, _P, _P, _P, _P, _i64, _P, _i64, _P, _i64],
+    "bsscl_grad_norm_workspace": [_i32, _P, _P],
+    "bsscl_grad_norm": [_i32, _P, _i32, _P, _P, _P, _f64, _P, _P, _i64],
+    "bsscl_clip_grads": [_i32, _P, _i32, _P, _P, _P, _P, _f64, _f64, _P, _P, _i64],
 }
 _VOID = {"bsscl_engine_destroy", "bsscl_sampler_destroy"}
 

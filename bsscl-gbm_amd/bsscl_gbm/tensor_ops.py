@@ -1,0 +1,234 @@
+"""Operators on device tensors: the softmax head over a large vocabulary with
+its gradient, and the norm and clipping of many tensors' gradients.
+
+They stand beside the estimator's softmax (which holds every score of up to 16
+classes) for class counts where the scores are too many to keep.  Inputs and
+outputs are torch tensors on one GPU; the kernels are libbsscl_hip.so's
+(``bsscl_head_*``, ``bsscl_grad_norm``, ``bsscl_clip_grads`` in
+include/bsscl_hip.h) and run on torch's current stream of that GPU.  Calls
+return without waiting for the GPU and can be captured into a HIP graph.
+Nothing is recorded for autograd: gradients are what the calls return.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from collections import namedtuple
+
+from . import _native
+
+__all__ = ["linear_softmax_loss", "linear_softmax_grad", "grad_norm", "clip_grads"]
+
+SoftmaxLoss = namedtuple("SoftmaxLoss", "loss row_loss lse")
+SoftmaxGrad = namedtuple("SoftmaxGrad", "loss row_loss lse d_hidden d_weight")
+
+_REDUCTIONS = {"sum": 0, "mean": 1}  # BSSCL_SUM, BSSCL_MEAN
+_dtype_codes = None
+
+
+def _torch():
+    """torch, which only these operators need, and the C ABI's dtype codes."""
+    global _dtype_codes
+    import torch
+    if _dtype_codes is None:
+        _dtype_codes = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    return torch
+
+
+def _stream(torch, device):
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _workspace(torch, device, fn, *args):
+    size = ctypes.c_int64()
+    _native.check(fn(*args, ctypes.byref(size)))
+    return torch.empty(size.value, dtype=torch.uint8, device=device)
+
+
+def _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, grad_scale):
+    torch = _torch()
+    if not (isinstance(hidden, torch.Tensor) and isinstance(weight, torch.Tensor)
+            and isinstance(labels, torch.Tensor)):
+        raise ValueError("hidden, weight and labels must be torch tensors")
+    code = _dtype_codes.get(hidden.dtype)
+    if code is None or weight.dtype != hidden.dtype:
+        raise ValueError("hidden and weight must both be bfloat16, float16 or float32, got "
+                         f"{hidden.dtype} and {weight.dtype}")
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hidden (..., width) and weight (vocab, width) do not fit: "
+                         f"{tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels {tuple(labels.shape)} must have the shape of hidden without its "
+                         f"last axis, {tuple(hidden.shape[:-1])}")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"labels must be int64 or int32, got {labels.dtype}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be 'mean' or 'sum', got {reduction!r}")
+    if row_weight is not None and (not isinstance(row_weight, torch.Tensor)
+                                   or row_weight.dtype != torch.float32
+                                   or row_weight.shape != labels.shape):
+        raise ValueError("row_weight must be a float32 tensor of the labels' shape")
+    dev = hidden.device
+    if dev.type != "cuda":
+        raise ValueError("hidden must be on a GPU")
+    for name, t in (("weight", weight), ("labels", labels), ("row_weight", row_weight)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, hidden on {dev}")
+    vocab, width = weight.shape
+    if vocab < 1 or width < 1:
+        raise ValueError("vocab and width must be at least 1")
+    rows = labels.numel()
+    grad = grad_scale is not None
+    f32 = dict(dtype=torch.float32, device=dev)
+    out = [torch.empty((), **f32), torch.empty(labels.shape, **f32),
+           torch.empty(labels.shape, **f32)]
+    if grad:
+        out += [torch.empty(hidden.shape, dtype=hidden.dtype, device=dev),
+                torch.empty(weight.shape, dtype=weight.dtype, device=dev)]
+    if rows == 0:
+        out[0].zero_()
+        if grad:
+            out[4].zero_()
+        return out
+    hidden = hidden.reshape(rows, width)
+    if width > 1 and hidden.stride(1) != 1 or rows > 1 and hidden.stride(0) < width:
+        hidden = hidden.contiguous()
+    if width > 1 and weight.stride(1) != 1 or vocab > 1 and weight.stride(0) < width:
+        weight = weight.contiguous()
+    labels = labels.reshape(rows).to(torch.int64).contiguous()
+    if row_weight is not None:
+        row_weight = row_weight.reshape(rows).contiguous()
+    h_stride = max(hidden.stride(0), width)  # a single row may have any stride
+    w_stride = max(weight.stride(0), width)
+    L = _native.lib()
+    ws = _workspace(torch, dev, L.bsscl_head_workspace, code, rows, width, vocab,
+                    weight.data_ptr(), w_stride, int(grad))
+    args = [dev.index, _stream(torch, dev), code, hidden.data_ptr(), h_stride, weight.data_ptr(),
+            w_stride, labels.data_ptr(), None if row_weight is None else row_weight.data_ptr(),
+            rows, width, vocab, _REDUCTIONS[reduction], float(softcap), float(z_loss)]
+    head = [t.data_ptr() for t in out[:3]]
+    if grad:
+        _native.check(L.bsscl_head_grad(*args, float(grad_scale), *head, out[3].data_ptr(), width,
+                                        out[4].data_ptr(), width, ws.data_ptr(), ws.numel()))
+    else:
+        _native.check(L.bsscl_head_loss(*args, *head, ws.data_ptr(), ws.numel()))
+    return out
+
+
+def linear_softmax_loss(hidden, weight, labels, *, row_weight=None, reduction="mean", softcap=0.0,
+                        z_loss=0.0):
+    """Softmax cross entropy of the scores hidden @ weight.T, without keeping
+    the scores.
+
+    hidden (..., width) and weight (vocab, width) are bfloat16, float16 or
+    float32; labels (...) int64 or int32.  A row whose label is outside
+    [0, vocab), such as -1 or -100, is left out: its loss and lse are 0,
+    whatever its hidden values are.  row_weight (...) float32 weighs the rows;
+    reduction "mean" divides by the counting rows' sum of weights, "sum" does
+    not.  softcap c > 0 puts c * tanh(s / c) in the place of each score, and
+    z_loss zeta adds zeta * lse^2 to each row's loss.
+
+    Returns (loss, row_loss, lse) in float32: the reduced loss, each row's
+    unweighted loss (for z_loss=0 the negative log-probability of its label)
+    and each row's log of the sum of exponentials.
+    """
+    return SoftmaxLoss(*_head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, None))
+
+
+def linear_softmax_grad(hidden, weight, labels, *, row_weight=None, reduction="mean", softcap=0.0,
+                        z_loss=0.0, grad_scale=1.0):
+    """linear_softmax_loss with its gradient: (loss, row_loss, lse, d_hidden,
+    d_weight).
+
+    d_hidden and d_weight are the gradients of the reduced loss times
+    grad_scale (the loss scale of a float16 run; clip_grads and grad_norm take
+    its inverse), in the inputs' dtype; rows left out have zeros.
+    """
+    return SoftmaxGrad(*_head(hidden, weight, labels, row_weight, reduction, softcap, z_loss,
+                              float(grad_scale)))
+
+
+def _dense(t):
+    """Whether t's values fill one block of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for stride, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True
+
+
+def _list(torch, tensors, what):
+    tensors = list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what} must be torch tensors, got {type(t).__name__}")
+    if not tensors:
+        raise ValueError(f"{what} is empty")
+    codes = [_dtype_codes.get(t.dtype, -1) for t in tensors]
+    if min(codes) < 0:
+        raise ValueError(f"{what} must be bfloat16, float16 or float32, got "
+                         f"{tensors[codes.index(-1)].dtype}")
+    dev = tensors[0].get_device()
+    if dev < 0 or any(t.get_device() != dev for t in tensors):
+        raise ValueError(f"{what} must all be on one GPU")
+    for t in tensors:
+        if not _dense(t):
+            raise ValueError(f"{what} must be dense: a tensor of shape {tuple(t.shape)} has "
+                             f"strides {t.stride()}")
+    return tensors, codes, dev
+
+
+def _norm(tensors, inv_scale, max_norm, out):
+    torch = _torch()
+    tensors, codes, dev = _list(torch, tensors, "tensors")
+    n = len(tensors)
+    ptrs = [t.data_ptr() for t in tensors]
+    outs = None
+    if max_norm is not None:
+        outs = ptrs
+        if out is not None:
+            out, out_codes, out_dev = _list(torch, out, "out")
+            if len(out) != n or out_codes != codes or out_dev != dev or any(
+                    o.shape != t.shape or o.stride() != t.stride() for o, t in zip(out, tensors)):
+                raise ValueError("out must match tensors in number, shape, strides, dtype and GPU")
+            outs = [t.data_ptr() for t in out]
+    lengths = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    codes = (ctypes.c_int32 * n)(*codes)
+    ptrs = (ctypes.c_void_p * n)(*ptrs)
+    dev = torch.device("cuda", dev)
+    L = _native.lib()
+    ws = _workspace(torch, dev, L.bsscl_grad_norm_workspace, n, lengths)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    args = (dev.index, _stream(torch, dev), n, ptrs)
+    if outs is None:
+        _native.check(L.bsscl_grad_norm(*args, lengths, codes, float(inv_scale), norm.data_ptr(),
+                                        ws.data_ptr(), ws.numel()))
+    else:
+        _native.check(L.bsscl_clip_grads(*args, (ctypes.c_void_p * n)(*outs), lengths, codes,
+                                         float(inv_scale), float(max_norm), norm.data_ptr(),
+                                         ws.data_ptr(), ws.numel()))
+    return norm
+
+
+def grad_norm(tensors, *, inv_scale=1.0):
+    """The 2-norm over all values of the tensors, times abs(inv_scale), as a
+    float32 tensor.  tensors: dense (in any order of axes) bfloat16, float16
+    or float32 tensors on one GPU, mixed and of any sizes."""
+    return _norm(tensors, inv_scale, None, None)
+
+
+def clip_grads(tensors, max_norm, *, inv_scale=1.0, out=None):
+    """Scales the tensors by inv_scale * min(1, max_norm / norm), where norm
+    is grad_norm(tensors, inv_scale=inv_scale), in place or into the tensors
+    of `out` (same shapes, strides and dtypes), and returns norm.
+
+    A norm that is NaN or infinite clips nothing (the factor is inv_scale):
+    look at the returned norm and skip the step.  Tensors to be written may
+    not overlap each other or another tensor."""
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f"max_norm must be >= 0, got {max_norm}")
+    return _norm(tensors, inv_scale, max_norm, out)

@@ -469,6 +469,85 @@ int bsscl_engine_set_profiling(bsscl_engine *eng, int32_t on);
 int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
                        int32_t *n_out);
 
+/*
+ * Operators on device buffers: the softmax head over a large set of classes
+ * with its gradient, and the norm and clipping of the gradients of many
+ * tensors.  No reference counterpart (its softmax, est:2327-2332, holds every
+ * score of a few classes).  They take device memory of GPU `device`, enqueue
+ * on `stream` (a hipStream_t, NULL for the default one) and return without
+ * waiting; they allocate nothing, keep nothing between calls and may be
+ * captured into a HIP graph.  `workspace` is device memory of at least the
+ * size that the matching _workspace call gives, aligned to 256 bytes, and
+ * belongs to the call until its work on the stream has ended: calls that can
+ * overlap need workspaces of their own.  Results do not depend on timing: the
+ * same call gives the same bits.
+ */
+#define BSSCL_BF16 0
+#define BSSCL_F16 1
+#define BSSCL_F32 2
+
+#define BSSCL_SUM 0   /* weights as they are */
+#define BSSCL_MEAN 1  /* weights divided by their sum over the counting rows */
+
+/*
+ * Softmax cross entropy of scores hidden x weight^T, in tiles: no score is
+ * ever written.
+ *   hidden      rows x width, row stride hidden_stride (elements)
+ *   weight      vocab x width, row stride weight_stride, of the same dtype
+ *   labels      int64[rows]; a row whose label is outside [0, vocab) is left
+ *               out: its outputs are 0 whatever its hidden values are
+ *   row_weight  float32[rows] or NULL for ones
+ *   softcap     c > 0: z = c tanh(s / c) in the place of each score s; 0: none
+ *   z_loss      zeta >= 0: each row's loss gets + zeta * lse^2
+ * With z the scores, lse = log sum exp z and u the row weights (reduction):
+ *   row_loss[i] = lse_i - z_i[label_i] + zeta lse_i^2,   loss = sum u_i row_loss[i]
+ * loss float32[1], row_loss and lse float32[rows].  A mean over weights whose
+ * sum is 0 (no counting row) is 0, with gradients of 0.
+ * bsscl_head_grad adds, times grad_scale,
+ *   d_hidden = d loss / d hidden (rows x width, stride d_hidden_stride) and
+ *   d_weight = d loss / d weight (vocab x width, stride d_weight_stride),
+ * both of the inputs' dtype and overwritten.
+ * Sums run in float32; d loss / d score is rounded to the inputs' dtype once
+ * it has been normalised, as operand of the two products.  In float16 it is
+ * scaled by a power of two first (it holds at least 2^-35 of the largest row
+ * weight), and 1 + 2 zeta lse may reach 32.
+ * 1 <= rows, vocab < 2^30; 1 <= width <= 65536.
+ */
+int bsscl_head_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t vocab,
+                         const void *weight, int64_t weight_stride, int32_t with_grad,
+                         int64_t *bytes);
+int bsscl_head_loss(int32_t device, void *stream, int32_t dtype, const void *hidden,
+                    int64_t hidden_stride, const void *weight, int64_t weight_stride,
+                    const int64_t *labels, const float *row_weight, int64_t rows, int64_t width,
+                    int64_t vocab, int32_t reduction, double softcap, double z_loss, float *loss,
+                    float *row_loss, float *lse, void *workspace, int64_t workspace_bytes);
+int bsscl_head_grad(int32_t device, void *stream, int32_t dtype, const void *hidden,
+                    int64_t hidden_stride, const void *weight, int64_t weight_stride,
+                    const int64_t *labels, const float *row_weight, int64_t rows, int64_t width,
+                    int64_t vocab, int32_t reduction, double softcap, double z_loss,
+                    double grad_scale, float *loss, float *row_loss, float *lse, void *d_hidden,
+                    int64_t d_hidden_stride, void *d_weight, int64_t d_weight_stride,
+                    void *workspace, int64_t workspace_bytes);
+
+/*
+ * The 2-norm over all values of count tensors (device pointers, lengths and
+ * dtypes in host arrays), and the tensors scaled to it:
+ *   norm = |inv_scale| sqrt(sum of squares)            (float32[1])
+ *   out[t][i] = tensors[t][i] * inv_scale * min(1, max_norm / norm)
+ * Squares are summed in float64 in a fixed order.  A norm that is NaN or
+ * infinite clips nothing (the factor is inv_scale): the caller sees it in
+ * `norm`.  out[t] may be tensors[t] itself; otherwise no out may overlap any
+ * tensor, and no two outs may overlap (refused).
+ */
+int bsscl_grad_norm_workspace(int32_t count, const int64_t *lengths, int64_t *bytes);
+int bsscl_grad_norm(int32_t device, void *stream, int32_t count, const void *const *tensors,
+                    const int64_t *lengths, const int32_t *dtypes, double inv_scale, float *norm,
+                    void *workspace, int64_t workspace_bytes);
+int bsscl_clip_grads(int32_t device, void *stream, int32_t count, const void *const *tensors,
+                     void *const *out, const int64_t *lengths, const int32_t *dtypes,
+                     double inv_scale, double max_norm, float *norm, void *workspace,
+                     int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif
