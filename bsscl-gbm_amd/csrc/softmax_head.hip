@@ -20,13 +20,12 @@
 #include <type_traits>
 
 #include "device_call.h"
+#include "mfma_tile.h"
 
 namespace bsscl {
 
 namespace {
 
-constexpr int kTileV = 64;      // classes of a score tile
-constexpr int kTileR = 64;      // rows of a score tile
 constexpr int kRowPad = 256;    // rows of a piece: a multiple
 constexpr int kColPad = 64;     // width of the packed rows: a multiple
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
@@ -168,76 +167,108 @@ __global__ __launch_bounds__(256) void k_pack_hidden(const T *hidden, int64_t st
   }
 }
 
-// 64 x 64 tile of sum_k A(m, k) B(n, k) in float32: thread (tx, ty) of 16 x 16
-// holds m = 4 ty + 0..3, n = 4 tx + 0..3.  A and B give 0 outside.
-template <typename FA, typename FB>
-__device__ void mm_tile(FA A, FB B, int64_t k_end, float (&acc)[4][4]) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int tx = (int)threadIdx.x & 15, ty = (int)threadIdx.x >> 4;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  for (int64_t k0 = 0; k0 < k_end; k0 += 16) {
-    for (int e = (int)threadIdx.x; e < 1024; e += 256) {
-      sa[e & 15][e >> 4] = A(e >> 4, k0 + (e & 15));
-      sb[e & 15][e >> 4] = B(e >> 4, k0 + (e & 15));
-    }
-    __syncthreads();
-    for (int k = 0; k < 16; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] += sa[k][4 * ty + i] * sb[k][4 * tx + j];
-    __syncthreads();
-  }
+// Tile `at` of slow x fast tiles: kGroup of the fast ones side by side, so that
+// the tiles that run together share operands on both sides.
+struct TileAt {
+  int32_t slow, fast;
+};
+__device__ __forceinline__ TileAt tile_at(uint32_t at, uint32_t slow, uint32_t fast) {
+  constexpr uint32_t kGroup = 8;
+  const uint32_t group = at / (slow * kGroup), in = at % (slow * kGroup);
+  const uint32_t width = min(kGroup, fast - group * kGroup);
+  return {(int32_t)(in / width), (int32_t)(group * kGroup + in % width)};
 }
 
-// One score tile: kTileV classes x kTileR rows.
-template <typename T>
-__global__ __launch_bounds__(256) void k_scores(const T *weight, int64_t w_stride, int32_t vocab,
-                                                int32_t width, const T *packed, int32_t wide,
-                                                const int32_t *lab, const HeadInfo *info,
-                                                int32_t piece, int32_t pieces, float softcap,
-                                                int32_t tiles, float2 *stats, float *z_label, T *P,
-                                                int64_t ldp) {
-  __shared__ float z[kTileR][kTileV + 1];
+// Score tiles: BM classes x BN rows.
+template <typename TL>
+__global__ __launch_bounds__(TL::kThreads) void k_scores(
+    const typename TL::T *weight, int64_t w_stride, int32_t vocab, int32_t width,
+    const typename TL::T *packed, int32_t wide, const int32_t *lab, const HeadInfo *info,
+    int32_t piece, int32_t pieces, float softcap, int32_t tiles, float2 *stats, float *z_label,
+    typename TL::T *P, int64_t ldp) {
+  using T = typename TL::T;
+  __shared__ __align__(1024) char lds[TL::kLdsOut];
   const Piece pc = piece_of(info->rows, piece, pieces);
-  const int32_t r0 = (int32_t)blockIdx.y * kTileR, v0 = (int32_t)blockIdx.x * kTileV;
-  if (r0 >= pc.rows) return;
-  const T *h = packed + ((int64_t)pc.begin + r0) * wide;
-  float acc[4][4];
-  mm_tile(
-      [&](int m, int64_t k) {
-        return v0 + m < vocab && k < width ? (float)weight[(int64_t)(v0 + m) * w_stride + k] : 0.f;
-      },
-      [&](int n, int64_t k) { return k < wide ? (float)h[(int64_t)n * wide + k] : 0.f; }, width, acc);
-  const int tx = (int)threadIdx.x & 15, ty = (int)threadIdx.x >> 4;
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      float s = acc[i][j];
-      if (softcap > 0.f) s = softcap * tanhf(s / softcap);
-      z[4 * tx + j][4 * ty + i] = v0 + 4 * ty + i < vocab ? s : -INFINITY;
-    }
-  __syncthreads();
-  const int n = (int)threadIdx.x;
-  if (n < kTileR) {
-    const int32_t r = r0 + n;
-    float m = -INFINITY, s = 0.f;
-    for (int v = 0; v < kTileV; ++v) m = fmaxf(m, z[n][v]);
-    if (r < pc.rows) {
-      const int32_t y = lab[pc.begin + r] - v0;
-      if (y >= 0 && y < kTileV) z_label[r] = z[n][y];
-    }
-    const float base = m == -INFINITY ? 0.f : m;
-    for (int v = 0; v < kTileV; ++v) {
-      const float zv = z[n][v], e = expf(zv - base);
-      s += e;
-      const float slope = softcap > 0.f && e > 0.f ? 1.f - (zv / softcap) * (zv / softcap) : 1.f;
-      z[n][v] = e * slope * kExpScale<T>;
-    }
-    if (r < pc.rows) stats[(int64_t)r * tiles + blockIdx.x] = make_float2(m, s);
+  const uint32_t row_tiles = (uint32_t)(pc.rows + TL::BN - 1) / TL::BN;
+  const uint32_t total = row_tiles * (uint32_t)tiles;
+  if (blockIdx.x >= total) return;
+  const TileAt at = tile_at(xcd_order(blockIdx.x, total), (uint32_t)tiles, row_tiles);
+  const int32_t v0 = at.slow * TL::BM, r0 = at.fast * TL::BN;
+  typename TL::A a;
+  typename TL::B b;
+  a.init(weight, w_stride, v0, vocab);
+  b.init(packed + (int64_t)pc.begin * wide, wide, r0, (pc.rows + kRowPad - 1) / kRowPad * kRowPad);
+  Acc16 acc[TL::MI][TL::NI] = {};
+  TL::walk(a, b, 0, width, lds, acc);
+
+  const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
+  const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
+  // A lane holds rows wn + 32 j + l % 32 and every fourth group of four
+  // classes; lanes l and l + 32 and the waves along m share a row.
+  float *part = reinterpret_cast<float *>(lds);  // [kWavesM][BN]
+  float top[TL::NI];
+#pragma unroll
+  for (int j = 0; j < TL::NI; ++j) {
+    const int n = wn + j * 32 + (l & 31);
+    const int32_t y = r0 + n < pc.rows ? lab[pc.begin + r0 + n] - v0 : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int v = wm + i * 32 + (r >> 2) * 8 + (l >> 5) * 4 + (r & 3);
+        float z = acc[i][j][r];
+        if (softcap > 0.f) z = softcap * tanhf(z / softcap);
+        z = v0 + v < vocab ? z : -INFINITY;
+        if (v == y) z_label[r0 + n] = z;
+        acc[i][j][r] = z;
+        m = fmaxf(m, z);
+      }
+    m = fmaxf(m, __shfl_xor(m, 32));
+    if (l < 32) part[wave / TL::kWavesN * TL::BN + n] = m;
   }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < TL::NI; ++j) {
+    float m = part[wn + j * 32 + (l & 31)];
+    for (int w = 1; w < TL::kWavesM; ++w) m = fmaxf(m, part[w * TL::BN + wn + j * 32 + (l & 31)]);
+    top[j] = m;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < TL::NI; ++j) {
+    const float base = top[j] == -INFINITY ? 0.f : top[j];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float z = acc[i][j][r], e = expf(z - base);
+        s += e;
+        if (P) {
+          const float t = softcap > 0.f && e > 0.f ? z / softcap : 0.f;
+          acc[i][j][r] = e * (1.f - t * t) * kExpScale<T>;
+        }
+      }
+    s += __shfl_xor(s, 32);
+    if (l < 32) part[wave / TL::kWavesN * TL::BN + wn + j * 32 + l] = s;
+  }
+  __syncthreads();
+  if (wm == 0 && l < 32)
+#pragma unroll
+    for (int j = 0; j < TL::NI; ++j) {
+      const int n = wn + j * 32 + l;
+      float s = part[n];
+      for (int w = 1; w < TL::kWavesM; ++w) s += part[w * TL::BN + n];
+      if (r0 + n < pc.rows) stats[(int64_t)(r0 + n) * tiles + at.slow] = make_float2(top[j], s);
+    }
   if (!P) return;
   __syncthreads();
-  for (int e = (int)threadIdx.x; e < kTileR * kTileV; e += 256)
-    P[(int64_t)(r0 + (e >> 6)) * ldp + v0 + (e & 63)] = (T)z[e >> 6][e & 63];
+  TL::stage_out(lds, [&](int i, int j, int r) { return (T)acc[i][j][r]; });
+  __syncthreads();
+  TL::read_out(lds, [&](int n, int m, Int4 x) {
+    *reinterpret_cast<Int4 *>(P + (int64_t)(r0 + n) * ldp + v0 + m) = x;
+  });
 }
 
 // One block per row of the piece: lse and loss from the tiles' statistics;
@@ -246,7 +277,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_rows(const HeadInfo *info, int32_t piece, int32_t pieces,
                                               const int32_t *idx, const int32_t *lab,
                                               const float *u, float softcap, float z_loss,
-                                              float grad_scale, int32_t tiles,
+                                              float grad_scale, int32_t tiles, int32_t tile_v,
                                               const float2 *stats, const float *z_label, T *P,
                                               int64_t ldp, float *row_loss, float *lse_out) {
   __shared__ float red[256];
@@ -293,71 +324,150 @@ __global__ __launch_bounds__(256) void k_rows(const HeadInfo *info, int32_t piec
   const float own = g * slope * (py + zl * (py + 1.f));
   T *row = P + (int64_t)r * ldp;
   for (int64_t v = tid; v < ldp; v += 256) {
-    const float f = expf(st[v / kTileV].x - lse) * (g * (1.f + zl) / kExpScale<T>);
+    const float f = expf(st[v / tile_v].x - lse) * (g * (1.f + zl) / kExpScale<T>);
     row[v] = from_float<T>(v == y ? own : (float)row[v] * f);
   }
 }
 
-// d_hidden of a piece: rows x width, over the whole vocabulary.
-template <typename T>
-__global__ __launch_bounds__(256) void k_d_hidden(const T *P, int64_t ldp, const T *weight,
-                                                  int64_t w_stride, int32_t vocab, int32_t width,
-                                                  const HeadInfo *info, int32_t piece,
-                                                  int32_t pieces, const int32_t *idx, T *d_hidden,
-                                                  int64_t d_stride) {
+// d_hidden of a piece: BM columns x BN rows over the `split`th part of the
+// vocabulary, as float32 sums of their own.
+template <typename TL>
+__global__ __launch_bounds__(TL::kThreads) void k_d_hidden(
+    const typename TL::T *P, int64_t ldp, const typename TL::T *weight, int64_t w_stride,
+    int32_t vocab, int32_t width, int32_t wide, const HeadInfo *info, int32_t piece,
+    int32_t pieces, int32_t splits, int32_t split_v, float *part, int64_t part_stride) {
+  __shared__ __align__(1024) char lds[TL::kLds];
   const Piece pc = piece_of(info->rows, piece, pieces);
-  const int32_t r0 = (int32_t)blockIdx.y * 64, d0 = (int32_t)blockIdx.x * 64;
-  if (r0 >= pc.rows) return;
-  float acc[4][4];
-  mm_tile(
-      [&](int m, int64_t k) {
-        return d0 + m < width && k < vocab ? (float)weight[k * w_stride + d0 + m] : 0.f;
-      },
-      [&](int n, int64_t k) { return k < vocab ? (float)P[(int64_t)(r0 + n) * ldp + k] : 0.f; },
-      vocab, acc);
-  const int tx = (int)threadIdx.x & 15, ty = (int)threadIdx.x >> 4;
-  for (int j = 0; j < 4; ++j) {
-    const int32_t r = r0 + 4 * tx + j;
+  const uint32_t row_tiles = (uint32_t)(pc.rows + TL::BN - 1) / TL::BN;
+  const uint32_t col_tiles = (uint32_t)(width + TL::BM - 1) / TL::BM;
+  const uint32_t each = row_tiles * col_tiles, total = each * (uint32_t)splits;
+  if (blockIdx.x >= total) return;
+  const uint32_t idx = xcd_order(blockIdx.x, total);
+  const TileAt at = tile_at(idx % each, col_tiles, row_tiles);
+  const int32_t d0 = at.slow * TL::BM, r0 = at.fast * TL::BN, split = (int32_t)(idx / each);
+  typename TL::A a;
+  typename TL::B b;
+  a.init(weight, w_stride, d0, width);
+  b.init(P, ldp, r0, (pc.rows + kRowPad - 1) / kRowPad * kRowPad);
+  Acc16 acc[TL::MI][TL::NI] = {};
+  TL::walk(a, b, (int64_t)split * split_v, min((int64_t)(split + 1) * split_v, (int64_t)vocab), lds,
+           acc);
+  const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
+  const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
+#pragma unroll
+  for (int j = 0; j < TL::NI; ++j) {
+    const int32_t r = r0 + wn + j * 32 + (l & 31);
     if (r >= pc.rows) continue;
-    T *out = d_hidden + (int64_t)idx[pc.begin + r] * d_stride;
-    for (int i = 0; i < 4; ++i)
-      if (d0 + 4 * ty + i < width) out[d0 + 4 * ty + i] = (T)(acc[i][j] * info->from_operand);
+    float *out = part + (int64_t)split * part_stride + (int64_t)r * wide;
+#pragma unroll
+    for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int32_t d = d0 + wm + i * 32 + q * 8 + (l >> 5) * 4;
+        if (d < wide)
+          *reinterpret_cast<float4 *>(out + d) =
+              make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                          acc[i][j][4 * q + 3]);
+      }
   }
 }
 
-// d_weight of a piece: vocab x width, over the piece's rows; pieces before the
-// last add up in float32.
+// The parts of d_hidden added up in their order, into the rows' places.
 template <typename T>
-__global__ __launch_bounds__(256) void k_d_weight(const T *P, int64_t ldp, const T *packed,
-                                                  int32_t wide, int32_t vocab, int32_t width,
-                                                  const HeadInfo *info, int32_t piece,
-                                                  int32_t pieces, float *sum, T *d_weight,
-                                                  int64_t d_stride) {
+__global__ __launch_bounds__(256) void k_d_hidden_sum(const HeadInfo *info, int32_t piece,
+                                                      int32_t pieces, const int32_t *idx,
+                                                      int32_t splits, const float *part,
+                                                      int64_t part_stride, int32_t wide,
+                                                      int32_t width, T *d_hidden,
+                                                      int64_t d_stride) {
   const Piece pc = piece_of(info->rows, piece, pieces);
-  const int32_t v0 = (int32_t)blockIdx.y * 64, d0 = (int32_t)blockIdx.x * 64;
-  const T *h = packed + (int64_t)pc.begin * wide;
-  float acc[4][4];
-  mm_tile(
-      [&](int m, int64_t k) {
-        return d0 + m < wide && k < pc.rows ? (float)h[k * wide + d0 + m] : 0.f;
-      },
-      [&](int n, int64_t k) { return k < pc.rows ? (float)P[k * ldp + v0 + n] : 0.f; }, pc.rows,
-      acc);
-  const int tx = (int)threadIdx.x & 15, ty = (int)threadIdx.x >> 4;
-  for (int j = 0; j < 4; ++j) {
-    const int32_t v = v0 + 4 * tx + j;
-    if (v >= vocab) continue;
-    for (int i = 0; i < 4; ++i) {
-      const int32_t d = d0 + 4 * ty + i;
-      if (d >= width) continue;
-      float x = acc[i][j];
-      if (piece > 0) x += sum[(int64_t)v * wide + d];
-      if (piece < pieces - 1)
-        sum[(int64_t)v * wide + d] = x;
-      else
-        d_weight[(int64_t)v * d_stride + d] = (T)(x * info->from_operand);
-    }
+  const int32_t r = (int32_t)blockIdx.x;
+  if (r >= pc.rows) return;
+  const float back = info->from_operand;
+  T *out = d_hidden + (int64_t)idx[pc.begin + r] * d_stride;
+  for (int32_t d = (int32_t)threadIdx.x; d < width; d += 256) {
+    const float *p = part + (int64_t)r * wide + d;
+    float s = 0.f;
+    for (int32_t k = 0; k < splits; ++k) s += p[(int64_t)k * part_stride];
+    out[d] = (T)(s * back);
   }
+}
+
+// d_weight of a piece: BM columns x BN classes over the piece's rows; pieces
+// before the last add up in float32.
+template <typename TL>
+__global__ __launch_bounds__(TL::kThreads) void k_d_weight(
+    const typename TL::T *P, int64_t ldp, const typename TL::T *packed, int32_t wide,
+    int32_t vocab, int32_t width, const HeadInfo *info, int32_t piece, int32_t pieces, float *sum,
+    typename TL::T *d_weight, int64_t d_stride, int32_t vec) {
+  using T = typename TL::T;
+  __shared__ __align__(1024) char lds[TL::kLdsOut];
+  const Piece pc = piece_of(info->rows, piece, pieces);
+  const uint32_t col_tiles = (uint32_t)(width + TL::BM - 1) / TL::BM;
+  const uint32_t v_tiles = (uint32_t)(vocab + TL::BN - 1) / TL::BN;
+  const TileAt at = tile_at(xcd_order(blockIdx.x, gridDim.x), v_tiles, col_tiles);
+  const int32_t v0 = at.slow * TL::BN, d0 = at.fast * TL::BM;
+  typename TL::A a;
+  typename TL::B b;
+  a.init(packed + (int64_t)pc.begin * wide, wide, d0, wide);
+  b.init(P, ldp, v0, (int32_t)ldp);
+  Acc16 acc[TL::MI][TL::NI] = {};
+  TL::walk(a, b, 0, (pc.rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
+  if (pieces > 1) {
+    const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
+    const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
+#pragma unroll
+    for (int j = 0; j < TL::NI; ++j) {
+      const int32_t v = v0 + wn + j * 32 + (l & 31);
+      if (v >= vocab) continue;
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int32_t d = d0 + wm + i * 32 + q * 8 + (l >> 5) * 4;
+          if (d >= wide) continue;
+          float4 *p = reinterpret_cast<float4 *>(sum + (int64_t)v * wide + d);
+          float4 x = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                                 acc[i][j][4 * q + 3]);
+          if (piece > 0) {
+            const float4 y = *p;
+            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+            acc[i][j][4 * q] = x.x;
+            acc[i][j][4 * q + 1] = x.y;
+            acc[i][j][4 * q + 2] = x.z;
+            acc[i][j][4 * q + 3] = x.w;
+          }
+          if (piece < pieces - 1) *p = x;
+        }
+    }
+    if (piece < pieces - 1) return;
+  }
+  const float back = info->from_operand;
+  TL::stage_out(lds, [&](int i, int j, int r) { return (T)(acc[i][j][r] * back); });
+  __syncthreads();
+  TL::read_out(lds, [&](int n, int m, Int4 x) {
+    if (v0 + n >= vocab) return;
+    T *out = d_weight + (int64_t)(v0 + n) * d_stride + d0 + m;
+    constexpr int kVec = 16 / (int)sizeof(T);
+    if (vec && d0 + m + kVec <= width) {
+      *reinterpret_cast<Int4 *>(out) = x;
+      return;
+    }
+    T e[kVec];
+    __builtin_memcpy(e, &x, 16);
+#pragma unroll
+    for (int k = 0; k < kVec; ++k)
+      if (d0 + m + k < width) out[k] = e[k];
+  });
+}
+
+// Rows of the weight at a stride and width that the tiles can load from.
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack_weight(const T *weight, int64_t stride,
+                                                     int32_t width, int32_t wide, T *packed) {
+  const int64_t v = (int64_t)blockIdx.x;
+  for (int32_t d = (int32_t)threadIdx.x; d < wide; d += 256)
+    packed[v * wide + d] = d < width ? weight[v * stride + d] : (T)0.f;
 }
 
 // loss = sum of u * row_loss over the counting rows, in their order.
@@ -372,33 +482,78 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const HeadInfo *info, const i
   if (threadIdx.x == 0) *loss = (float)s;
 }
 
+// The tile shapes: 256 x 256 fills the matrix cores best and needs a whole
+// CU's LDS; 128 x 128 gives four times the workgroups; 128 x 32 wastes less
+// where there are few rows.
+enum Shape : int32_t { kBig, kMid, kThin };
+template <typename T, Shape S, bool A_ACROSS, bool B_ACROSS>
+using TileOf = std::conditional_t<
+    S == kBig, Tile<T, 256, 256, 128, 64, A_ACROSS, B_ACROSS>,
+    std::conditional_t<S == kMid, Tile<T, 128, 128, 64, 64, A_ACROSS, B_ACROSS>,
+                       Tile<T, 128, 32, 32, 32, A_ACROSS, B_ACROSS>>>;
+constexpr int shape_m(Shape s) { return s == kBig ? 256 : 128; }
+constexpr int shape_n(Shape s) { return s == kBig ? 256 : s == kMid ? 128 : 32; }
+
+int64_t tiles_of(Shape s, int64_t m, int64_t n) {
+  return ((m + shape_m(s) - 1) / shape_m(s)) * ((n + shape_n(s) - 1) / shape_n(s));
+}
+
+constexpr int64_t kCus = 256;
+
 // Where a call's intermediate values lie in its workspace.
 struct HeadPlan {
-  int32_t rows, width, wide, vocab, tiles;
-  int32_t piece_rows, pieces;
+  int32_t rows, width, wide, vocab, tiles, tile_v;
+  int32_t piece_rows, pieces, splits, split_v;
+  Shape scores, d_hidden, d_weight;
+  bool pack_weight;
   int64_t ldp;
-  size_t info, idx, lab, u, pos, packed, stats, z_label, P, sum, bytes;
+  size_t info, idx, lab, u, pos, packed, stats, z_label, P, part, sum, weight, bytes;
 };
 
-int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, bool grad, HeadPlan *pl) {
+int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const void *weight,
+              int64_t w_stride, bool grad, HeadPlan *pl) {
   if (dtype != BSSCL_BF16 && dtype != BSSCL_F16 && dtype != BSSCL_F32)
     return set_error(BSSCL_EINVAL, "softmax head: unknown dtype " + std::to_string(dtype));
-  if (rows < 1 || vocab < 1 || width < 1 || rows >= (1 << 30) || vocab >= (1 << 30) ||
-      width > 65536)
+  if (rows < 1 || vocab < 1 || width < 1 || rows >= (1 << 30) || vocab > 4000000 || width > 65536)
     return set_error(BSSCL_EINVAL,
-                     "softmax head: rows and vocab must be in [1, 2^30), width in [1, 65536]");
-  const int64_t es = dtype == BSSCL_F32 ? 4 : 2;
+                     "softmax head: rows must be in [1, 2^30), vocab in [1, 4000000], width in "
+                     "[1, 65536]");
+  const bool f32 = dtype == BSSCL_F32;
+  const int64_t es = f32 ? 4 : 2;
   HeadPlan p{};
   p.rows = (int32_t)rows;
   p.width = (int32_t)width;
   p.wide = (int32_t)round_up(width, kColPad);
   p.vocab = (int32_t)vocab;
-  p.tiles = (int32_t)((vocab + kTileV - 1) / kTileV);
-  p.ldp = (int64_t)p.tiles * kTileV;
+  auto shape = [&](int64_t m, int64_t n) {
+    if (n <= 32) return kThin;
+    return !f32 && tiles_of(kBig, m, n) >= kCus ? kBig : kMid;
+  };
+  p.scores = shape(vocab, rows);
+  p.tile_v = shape_m(p.scores);
+  p.tiles = (int32_t)((vocab + p.tile_v - 1) / p.tile_v);
+  p.ldp = (int64_t)p.tiles * p.tile_v;
   const int64_t row_bytes = grad ? p.ldp * es : (int64_t)p.tiles * (int64_t)sizeof(float2);
   const int64_t fit = std::max<int64_t>(kRowPad, kPieceBytes / row_bytes / kRowPad * kRowPad);
   p.piece_rows = (int32_t)std::min<int64_t>(fit, round_up(rows, kRowPad));
   p.pieces = (int32_t)((rows + p.piece_rows - 1) / p.piece_rows);
+  if (grad) {
+    const int64_t piece = std::min<int64_t>(rows, p.piece_rows);
+    // d_hidden's sums run over the whole vocabulary: parts of it fill the CUs
+    // (four rounds of them, so that the last one weighs little), each of at
+    // least 16 steps.
+    p.d_hidden = piece <= 32 ? kThin : !f32 && width >= 256 && piece >= 256 ? kBig : kMid;
+    const int64_t step = kStepBytes / es, steps = (vocab + step - 1) / step;
+    const int64_t want = (4 * kCus + tiles_of(p.d_hidden, width, piece) - 1) /
+                         tiles_of(p.d_hidden, width, piece);
+    const int64_t splits = std::max<int64_t>(1, std::min(want, steps / 16));
+    p.split_v = (int32_t)((steps + splits - 1) / splits * step);
+    p.splits = (int32_t)((vocab + p.split_v - 1) / p.split_v);
+    p.d_weight = !f32 && tiles_of(kBig, width, vocab) >= kCus ? kBig : kMid;
+  }
+  // Loads are of 16 bytes, within 2^31 bytes of a tile's first row.
+  p.pack_weight = ((uintptr_t)weight & 15) || w_stride * es % 16 || width * es % 16 ||
+                  w_stride * es * 256 >= (int64_t(1) << 31);
   size_t at = 0;
   auto take = [&](int64_t bytes) {
     const size_t here = at;
@@ -414,7 +569,9 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, bool gr
   p.stats = take((int64_t)p.piece_rows * p.tiles * (int64_t)sizeof(float2));
   p.z_label = take((int64_t)p.piece_rows * 4);
   p.P = take(grad ? (int64_t)p.piece_rows * p.ldp * es : 0);
+  p.part = take(grad ? (int64_t)p.splits * p.piece_rows * p.wide * 4 : 0);
   p.sum = take(grad && p.pieces > 1 ? vocab * p.wide * 4 : 0);
+  p.weight = take(p.pack_weight ? vocab * p.wide * es : 0);
   p.bytes = at;
   *pl = p;
   return BSSCL_OK;
@@ -433,6 +590,17 @@ struct HeadCall {
   char *ws;
 };
 
+// f(std::integral_constant<Shape, s>) for s; float32 has no 256 x 256 tile
+// (its output would not fit LDS).
+template <typename T, bool THIN, typename F>
+void by_shape(Shape s, F &&f) {
+  if constexpr (sizeof(T) == 2)
+    if (s == kBig) return f(std::integral_constant<Shape, kBig>());
+  if constexpr (THIN)
+    if (s == kThin) return f(std::integral_constant<Shape, kThin>());
+  f(std::integral_constant<Shape, kMid>());
+}
+
 template <typename T>
 int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
   auto *info = reinterpret_cast<HeadInfo *>(c.ws + p.info);
@@ -444,30 +612,54 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
   auto *stats = reinterpret_cast<float2 *>(c.ws + p.stats);
   auto *z_label = reinterpret_cast<float *>(c.ws + p.z_label);
   auto *P = c.grad ? reinterpret_cast<T *>(c.ws + p.P) : nullptr;
+  auto *part = reinterpret_cast<float *>(c.ws + p.part);
   auto *sum = reinterpret_cast<float *>(c.ws + p.sum);
   auto *weight = static_cast<const T *>(c.weight);
+  int64_t w_stride = c.w_stride;
+  int32_t w_width = p.width;
+  if (p.pack_weight) {
+    auto *w = reinterpret_cast<T *>(c.ws + p.weight);
+    k_pack_weight<T><<<(unsigned)p.vocab, 256, 0, st>>>(weight, w_stride, p.width, p.wide, w);
+    weight = w;
+    w_stride = w_width = p.wide;
+  }
   k_head_prepare<<<1, 1024, 0, st>>>(c.labels, c.row_weight, p.rows, p.vocab, c.mean,
                                      c.grad_scale, std::is_same<T, _Float16>::value, idx, lab, u,
                                      pos, c.row_loss, c.lse, info);
-  k_pack_hidden<T><<<p.rows + kRowPad, 256, 0, st>>>(
+  k_pack_hidden<T><<<(unsigned)p.rows + kRowPad, 256, 0, st>>>(
       static_cast<const T *>(c.hidden), c.h_stride, p.rows, p.width, p.wide, pos, info, packed,
       static_cast<T *>(c.d_hidden), c.dh_stride);
+  const int64_t piece = std::min<int64_t>(p.rows, p.piece_rows);
+  const int64_t part_stride = (int64_t)p.piece_rows * p.wide;
+  const int vec = ((uintptr_t)c.d_weight & 15) == 0 && c.dw_stride * (int64_t)sizeof(T) % 16 == 0;
   for (int32_t k = 0; k < p.pieces; ++k) {
-    const unsigned row_tiles = (unsigned)(p.piece_rows / kTileR);
-    k_scores<T><<<dim3((unsigned)p.tiles, row_tiles), 256, 0, st>>>(
-        weight, c.w_stride, p.vocab, p.width, packed, p.wide, lab, info, k, p.pieces, c.softcap,
-        p.tiles, stats, z_label, P, p.ldp);
-    k_rows<T><<<p.piece_rows, 256, 0, st>>>(info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss,
-                                            c.grad_scale, p.tiles, stats, z_label, P, p.ldp,
-                                            c.row_loss, c.lse);
+    by_shape<T, true>(p.scores, [&](auto s) {
+      using TL = TileOf<T, decltype(s)::value, false, false>;
+      k_scores<TL><<<(unsigned)tiles_of(s, p.vocab, piece), TL::kThreads, 0, st>>>(
+          weight, w_stride, p.vocab, w_width, packed, p.wide, lab, info, k, p.pieces, c.softcap,
+          p.tiles, stats, z_label, P, p.ldp);
+    });
+    k_rows<T><<<(unsigned)(c.grad ? p.piece_rows : piece), 256, 0, st>>>(
+        info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
+        z_label, P, p.ldp, c.row_loss, c.lse);
     if (!c.grad) continue;
-    const unsigned cols = (unsigned)((p.width + 63) / 64);
-    k_d_hidden<T><<<dim3(cols, row_tiles), 256, 0, st>>>(P, p.ldp, weight, c.w_stride, p.vocab,
-                                                         p.width, info, k, p.pieces, idx,
-                                                         static_cast<T *>(c.d_hidden), c.dh_stride);
-    k_d_weight<T><<<dim3(cols, (unsigned)p.tiles), 256, 0, st>>>(
-        P, p.ldp, packed, p.wide, p.vocab, p.width, info, k, p.pieces, sum,
-        static_cast<T *>(c.d_weight), c.dw_stride);
+    by_shape<T, true>(p.d_hidden, [&](auto s) {
+      using TL = TileOf<T, decltype(s)::value, true, false>;
+      k_d_hidden<TL><<<(unsigned)(tiles_of(s, w_width, piece) * p.splits), TL::kThreads, 0, st>>>(P, p.ldp, weight, w_stride, p.vocab, w_width,
+                                                p.wide, info, k, p.pieces, p.splits, p.split_v,
+                                                part, part_stride);
+    });
+    k_d_hidden_sum<T><<<(unsigned)piece, 256, 0, st>>>(info, k, p.pieces, idx, p.splits, part,
+                                                       part_stride, p.wide, p.width,
+                                                       static_cast<T *>(c.d_hidden), c.dh_stride);
+    by_shape<T, false>(p.d_weight, [&](auto s) {
+      using TL = TileOf<T, decltype(s)::value, true, true>;
+      k_d_weight<TL><<<(unsigned)tiles_of(s, p.width, 1) *
+                           (unsigned)((p.vocab + TL::BN - 1) / TL::BN),
+                       TL::kThreads, 0, st>>>(
+          P, p.ldp, packed, p.wide, p.vocab, p.width, info, k, p.pieces, sum,
+          static_cast<T *>(c.d_weight), c.dw_stride, vec);
+    });
   }
   k_loss_sum<<<1, 1024, 0, st>>>(info, idx, u, c.row_loss, c.loss);
   const hipError_t e = hipGetLastError();
@@ -479,7 +671,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
 int head(int32_t device, void *stream, int32_t dtype, int64_t rows, int64_t width, int64_t vocab,
          int32_t reduction, int64_t workspace_bytes, const HeadCall &c) {
   HeadPlan p;
-  const int rc = head_plan(dtype, rows, width, vocab, c.grad, &p);
+  const int rc = head_plan(dtype, rows, width, vocab, c.weight, c.w_stride, c.grad, &p);
   if (rc != BSSCL_OK) return rc;
   if (!c.hidden || !c.weight || !c.labels || !c.loss || !c.row_loss || !c.lse || !c.ws ||
       (c.grad && (!c.d_hidden || !c.d_weight)))
@@ -521,7 +713,8 @@ int bsscl_head_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t voc
   return no_throw([&] {
     if (!bytes) return set_error(BSSCL_EINVAL, "softmax head: null argument");
     HeadPlan p;
-    const int rc = head_plan(dtype, rows, width, vocab, with_grad != 0, &p);
+    const int rc = head_plan(dtype, rows, width, vocab, weight, weight_stride, with_grad != 0,
+                             &p);
     if (rc == BSSCL_OK) *bytes = (int64_t)p.bytes;
     return rc;
   });
