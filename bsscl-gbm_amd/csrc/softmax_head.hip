@@ -26,6 +26,7 @@ namespace bsscl {
 
 namespace {
 
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kRowPad = 256;    // rows of a piece: a multiple
 constexpr int kColPad = 64;     // width of the packed rows: a multiple
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float z = acc[i][j][r], e = expf(z - base);
+        const float z = acc[i][j][r], e = __builtin_amdgcn_exp2f((z - base) * kLog2E);
         s += e;
         if (P) {
           const float t = softcap > 0.f && e > 0.f ? z / softcap : 0.f;
@@ -271,46 +272,74 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
   });
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) v = fmaxf(v, __shfl_xor(v, k));
+  return v;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) v += __shfl_xor(v, k);
+  return v;
+}
+
+// lse of a row from its tiles' statistics, by the block's kRowThreads threads.
+constexpr int kRowThreads = 256;
+__device__ float row_lse(const float2 *st, int32_t tiles, float *red) {
+  constexpr int kWaves = kRowThreads / 64;
+  const int tid = (int)threadIdx.x, wid = tid >> 6;
+  // Each thread's own maximum and sum first, rescaled as the maximum grows.
+  float m = -INFINITY, s = 0.f;
+  for (int t = tid; t < tiles; t += kRowThreads) {
+    const float2 x = st[t];
+    if (x.x > m) {
+      s = m == -INFINITY ? x.y : s * expf(m - x.x) + x.y;
+      m = x.x;
+    } else if (x.x != -INFINITY) {
+      s += x.y * expf(x.x - m);
+    } else {
+      s += x.y;  // NaN stays NaN
+    }
+  }
+  float top = wave_max(m);
+  if ((tid & 63) == 0) red[wid] = top;
+  __syncthreads();
+  top = red[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, red[w]);
+  s = wave_add(m == -INFINITY ? s : s * expf(m - top));
+  if ((tid & 63) == 0) red[kWaves + wid] = s;
+  __syncthreads();
+  s = red[kWaves];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) s += red[kWaves + w];
+  return (top == -INFINITY ? 0.f : top) + logf(s);
+}
+
 // One block per row of the piece: lse and loss from the tiles' statistics;
-// with P, the row of d loss / d score in its place.
+// with P, the row of d loss / d score in its place.  Bound by memory with P: a
+// block keeps kVecs 16-byte loads a thread in flight.
 template <typename T>
-__global__ __launch_bounds__(256) void k_rows(const HeadInfo *info, int32_t piece, int32_t pieces,
-                                              const int32_t *idx, const int32_t *lab,
-                                              const float *u, float softcap, float z_loss,
-                                              float grad_scale, int32_t tiles, int32_t tile_v,
-                                              const float2 *stats, const float *z_label, T *P,
-                                              int64_t ldp, float *row_loss, float *lse_out) {
-  __shared__ float red[256];
+__global__ __launch_bounds__(kRowThreads) void k_rows(
+    const HeadInfo *info, int32_t piece, int32_t pieces, const int32_t *idx, const int32_t *lab,
+    const float *u, float softcap, float z_loss, float grad_scale, int32_t tiles, int32_t tile_v,
+    const float2 *stats, const float *z_label, T *P, int64_t ldp, float *row_loss,
+    float *lse_out) {
+  __shared__ float red[2 * kRowThreads / 64];
+  constexpr int kVec = 16 / (int)sizeof(T), kVecs = 4;
   const Piece pc = piece_of(info->rows, piece, pieces);
   const int32_t r = (int32_t)blockIdx.x;
   const int tid = (int)threadIdx.x;
+  Int4 *row = reinterpret_cast<Int4 *>(P + (int64_t)r * ldp);
+  const int32_t n = (int32_t)(ldp / kVec);
   if (r >= pc.rows) {
     // The products read whole steps of rows: zeros behind the last one.
     if (P && r < (pc.rows + kRowPad - 1) / kRowPad * kRowPad)
-      for (int64_t v = tid; v < ldp; v += 256) P[(int64_t)r * ldp + v] = (T)0.f;
+      for (int32_t i = tid; i < n; i += kRowThreads) row[i] = Int4{0, 0, 0, 0};
     return;
   }
   const float2 *st = stats + (int64_t)r * tiles;
-  float m = -INFINITY;
-  for (int t = tid; t < tiles; t += 256) m = fmaxf(m, st[t].x);
-  red[tid] = m;
-  for (int k = 128; k > 0; k >>= 1) {
-    __syncthreads();
-    if (tid < k) red[tid] = fmaxf(red[tid], red[tid + k]);
-  }
-  __syncthreads();
-  m = red[0];
-  const float base = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  for (int t = tid; t < tiles; t += 256) s += st[t].y * expf(st[t].x - base);
-  __syncthreads();
-  red[tid] = s;
-  for (int k = 128; k > 0; k >>= 1) {
-    __syncthreads();
-    if (tid < k) red[tid] += red[tid + k];
-  }
-  __syncthreads();
-  const float lse = base + logf(red[0]);
+  const float lse = row_lse(st, tiles, red);
   const int32_t c = pc.begin + r, y = lab[c];
   const float zy = z_label[r];
   if (tid == 0) {
@@ -322,10 +351,31 @@ __global__ __launch_bounds__(256) void k_rows(const HeadInfo *info, int32_t piec
   const float py = expm1f(zy - lse);
   const float slope = softcap > 0.f ? 1.f - (zy / softcap) * (zy / softcap) : 1.f;
   const float own = g * slope * (py + zl * (py + 1.f));
-  T *row = P + (int64_t)r * ldp;
-  for (int64_t v = tid; v < ldp; v += 256) {
-    const float f = expf(st[v / tile_v].x - lse) * (g * (1.f + zl) / kExpScale<T>);
-    row[v] = from_float<T>(v == y ? own : (float)row[v] * f);
+  const float scale = g * (1.f + zl) / kExpScale<T>;
+  const int tile_shift = 31 - __clz(tile_v / kVec);
+  for (int32_t i0 = tid; i0 < n; i0 += kRowThreads * kVecs) {
+    Int4 x[kVecs];
+    float f[kVecs];
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int32_t i = i0 + k * kRowThreads;
+      if (i < n) {
+        x[k] = row[i];
+        f[k] = st[i >> tile_shift].x;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int32_t i = i0 + k * kRowThreads;
+      if (i >= n) continue;
+      const float by = expf(f[k] - lse) * scale;
+      typedef T TV __attribute__((ext_vector_type(kVec)));
+      TV v = __builtin_bit_cast(TV, x[k]);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        v[e] = from_float<T>(i * kVec + e == y ? own : (float)v[e] * by);
+      row[i] = __builtin_bit_cast(Int4, v);
+    }
   }
 }
 
@@ -639,7 +689,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
           weight, w_stride, p.vocab, w_width, packed, p.wide, lab, info, k, p.pieces, c.softcap,
           p.tiles, stats, z_label, P, p.ldp);
     });
-    k_rows<T><<<(unsigned)(c.grad ? p.piece_rows : piece), 256, 0, st>>>(
+    k_rows<T><<<(unsigned)(c.grad ? p.piece_rows : piece), kRowThreads, 0, st>>>(
         info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
         z_label, P, p.ldp, c.row_loss, c.lse);
     if (!c.grad) continue;
