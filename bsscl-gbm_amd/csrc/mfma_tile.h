@@ -2,14 +2,11 @@
 // bf16, fp16 and float32 operands with float32 sums.
 //
 // A workgroup holds a BM x BN tile in registers, WM x WN per wave in blocks of
-// 32 x 32 (v_mfma 32x32x16, for float32 32x32x2), and walks k in steps of 128
-// bytes.  Both operands' steps go from memory straight to LDS (buffer loads
-// with the lds bit: no registers), into one of two buffers while the other one
-// is read; a step takes one barrier.  An operand lies in memory with k
-// contiguous (rows of m or n) or with m or n contiguous (rows of k):
-//   k contiguous   LDS rows of 128 bytes, 16-byte chunk c of row r in place
-//                  c ^ (r & 7): eight lanes that read one chunk of eight rows
-//                  touch all eight places, so no bank twice
+// 32 x 32 (v_mfma 32x32x16, for float32 32x32x2), and walks k in steps.  Both
+// operands' steps go from memory straight to LDS (buffer loads with the lds
+// bit: no registers), into a ring of buffers.  An operand lies in memory with
+// k contiguous (rows of m or n) or with m or n contiguous (rows of k):
+//   k contiguous   LDS rows of one step's bytes; a lane reads 16 bytes of a row
 //   k across rows  LDS rows of the tile's m (n) range; 16-bit fragments come
 //                  from transposing reads (ds_read_b64_tr_b16: a group of 16
 //                  lanes reads 4 k x 16 m and gets k in registers), and chunk
@@ -37,7 +34,6 @@ typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 F16x8 __attribute__((ext_vector_type(8)));
 typedef short Short4 __attribute__((ext_vector_type(4)));
 
-constexpr int kStepBytes = 128;          // of k in one step
 constexpr uint32_t kNoRead = 0x80000000u;  // a lane's offset beyond every bound
 
 // acc += a b over one 16-byte fragment of k.
@@ -74,17 +70,28 @@ __device__ __forceinline__ Int4 buffer_of(const char *base, uint32_t bytes) {
   return Int4{(int)(uint32_t)a, (int)(uint32_t)(a >> 32), (int)bytes, 0x00020000};
 }
 
-// One operand of a tile: MN rows (columns) of C, `across`: k across rows.
-template <typename T, int MN, bool ACROSS, int WAVES>
+// One operand of a tile: MN rows (columns) of C, `across`: k across rows;
+// STEP: bytes of k in one step.
+template <typename T, int MN, bool ACROSS, int WAVES, int STEP>
 struct Operand {
   static constexpr int kES = (int)sizeof(T);
-  static constexpr int kStep = kStepBytes / kES;  // k of one step
-  static constexpr int kBytes = MN * kStepBytes;  // LDS of one step
-  static constexpr int kRowBytes = ACROSS ? MN * kES : kStepBytes;
+  static constexpr int kStep = STEP / kES;  // k of one step
+  static constexpr int kBytes = MN * STEP;  // LDS of one step
+  static constexpr int kRowBytes = ACROSS ? MN * kES : STEP;
   static constexpr int kChunks = kRowBytes / 16;  // of an LDS row
   static constexpr int kRowsPerLoad = 64 / kChunks;
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // of each wave in a step
   static_assert(kLoads >= 1 && kLoads * 1024 * WAVES == kBytes && kChunks <= 64, "tile shape");
+
+  // The place of chunk c of LDS row r.  Sixteen lanes read 16 bytes each in one
+  // go: with k contiguous, of one chunk of 16 rows, which lie in all 16
+  // chunks of a bank line (256 bytes: kPerLine rows).
+  static constexpr int kPerLine = 256 / kRowBytes > 0 ? 256 / kRowBytes : 1;
+  __device__ static __forceinline__ int place_of(int c, int r) {
+    if constexpr (!ACROSS) return c ^ ((r / kPerLine) & (kChunks - 1));
+    else if constexpr (kES == 2) return c ^ (((r & 3) * 4) & (kChunks - 1));
+    else return c;
+  }
 
   const char *base;
   int64_t stride;  // bytes from row to row
@@ -104,11 +111,10 @@ struct Operand {
     for (int i = 0; i < kLoads; ++i) {
       const int row = (i * WAVES + wave) * kRowsPerLoad + lane / kChunks;
       const int place = lane % kChunks;
+      chunk = (uint32_t)place_of(place, row);  // its own inverse
       if constexpr (!ACROSS) {
-        chunk = (uint32_t)(place ^ (row & 7));
         offset[i] = (uint32_t)(row * stride) + chunk * 16;
       } else {
-        chunk = (uint32_t)(kES == 2 ? place ^ (((row & 3) * 4) & (kChunks - 1)) : place);
         offset[i] = (int)(chunk * (16 / kES)) < valid ? (uint32_t)(row * stride) + chunk * 16
                                                       : kNoRead;
       }
@@ -121,7 +127,7 @@ struct Operand {
     const uint32_t at = lds_at + ((uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) << 10);
     if constexpr (!ACROSS) {
       // (Rows are padded to whole chunks.)
-      const int32_t bytes = (int32_t)min((left * kES + 15) & ~int64_t(15), (int64_t)kStepBytes);
+      const int32_t bytes = (int32_t)min((left * kES + 15) & ~int64_t(15), (int64_t)STEP);
       const Int4 r = buffer_of(base + k * kES,
                                valid > 0 ? (uint32_t)((valid - 1) * stride) + (uint32_t)bytes : 0);
 #pragma unroll
@@ -137,16 +143,16 @@ struct Operand {
     }
   }
 
-  // The fragment of k part `part` (of 4) and the 32 rows from `first` on.
+  // The fragment of k part `part` (of STEP / 32) and the 32 rows from `first` on.
   __device__ static __forceinline__ Int4 fragment(const char *lds, int first, int part) {
     const int l = (int)threadIdx.x & 63;
     if constexpr (!ACROSS) {
-      return *reinterpret_cast<const Int4 *>(lds + (first + (l & 31)) * kStepBytes +
-                                             (((part * 2 + (l >> 5)) ^ (l & 7)) << 4));
+      return *reinterpret_cast<const Int4 *>(lds + (first + (l & 31)) * STEP +
+                                             (place_of(part * 2 + (l >> 5), l & 31) << 4));
     } else if constexpr (kES == 2) {
       const int k = part * 16 + (l >> 5) * 8 + ((l & 15) >> 2);
       const int m = first + ((l >> 4) & 1) * 16 + (l & 3) * 4;
-      const int c = (m >> 3) ^ (((k & 3) * 4) & (kChunks - 1));
+      const int c = place_of(m >> 3, k);
       const char *p = lds + k * kRowBytes + (c << 4) + (m & 4) * 2;
       typedef __attribute__((address_space(3))) Short4 *LdsShort4;
       const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(p));
@@ -163,58 +169,90 @@ struct Operand {
   }
 };
 
-// A tile's shape: BM x BN per workgroup, WM x WN per wave.
-template <typename T_, int BM_, int BN_, int WM_, int WN_, bool A_ACROSS, bool B_ACROSS>
+template <int VM>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(VM) : "memory");
+}
+
+// A tile's shape: BM x BN per workgroup, WM x WN per wave; STEP bytes of k at
+// a time, STAGES (at least 3) of them in LDS.
+template <typename T_, int BM_, int BN_, int WM_, int WN_, bool A_ACROSS, bool B_ACROSS, int STEP,
+          int STAGES>
 struct Tile {
   using T = T_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int kWavesM = BM / WM, kWavesN = BN / WN, kWaves = kWavesM * kWavesN;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int MI = WM / 32, NI = WN / 32;
-  using A = Operand<T, BM, A_ACROSS, kWaves>;
-  using B = Operand<T, BN, B_ACROSS, kWaves>;
-  static constexpr int kStep = A::kStep;
+  using A = Operand<T, BM, A_ACROSS, kWaves, STEP>;
+  using B = Operand<T, BN, B_ACROSS, kWaves, STEP>;
+  static constexpr int kStep = A::kStep, kParts = STEP / 32;
   static constexpr int kStage = A::kBytes + B::kBytes;
-  static constexpr int kLds = 2 * kStage;
-  static_assert(kLds <= 160 * 1024, "two steps fit LDS");
+  static constexpr int kLds = STAGES * kStage;
+  static_assert(kLds <= 160 * 1024 && STAGES >= 3 && kParts % 2 == 0, "tile shape");
 
   // acc[mi][ni] += products of k in [k_begin, k_end); k_begin is a multiple of
   // kStep.  Every thread of the workgroup calls it; LDS is free at its end.
+  //
+  // Step k is read while those up to k + STAGES - 1 load: A's part of the last
+  // one is issued at the step's beginning, B's in its last part (all at once,
+  // every wave would wait for the address units while the matrix cores idle).
+  // Fragments are read one part ahead of the products that use them, the first
+  // part of a step during the last products of the step before: there stands
+  // the step's one barrier, when every wave has read the last of its buffer
+  // and the next step's own loads have landed.
   __device__ static __forceinline__ void walk(const A &a, const B &b, int64_t k_begin,
                                               int64_t k_end, char *lds, Acc16 (&acc)[MI][NI]) {
     const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / kWavesN * WM, wn = wave % kWavesN * WN;
     const uint32_t lds_at =
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    if (k_begin < k_end) {
-      a.load(k_begin, k_end, lds_at);
-      b.load(k_begin, k_end, lds_at + A::kBytes);
-    }
-    int buf = 0;
-    for (int64_t k = k_begin; k < k_end; k += kStep, buf ^= 1) {
-      // This step's loads have landed and every wave is done with the other
-      // buffer.
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k + kStep < k_end) {
-        const uint32_t at = lds_at + (uint32_t)((buf ^ 1) * kStage);
-        a.load(k + kStep, k_end, at);
-        b.load(k + kStep, k_end, at + A::kBytes);
-      }
+    Int4 fa[2][MI], fb[2][NI];
+    auto read = [&](int buf, int part, int set) {
       const char *cur = lds + buf * kStage;
 #pragma unroll
-      for (int part = 0; part < 4; ++part) {
-        Int4 fa[MI], fb[NI];
+      for (int j = 0; j < NI; ++j) fb[set][j] = B::fragment(cur + A::kBytes, wn + j * 32, part);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[i] = A::fragment(cur, wm + i * 32, part);
+      for (int i = 0; i < MI; ++i) fa[set][i] = A::fragment(cur, wm + i * 32, part);
+    };
+    auto load_a = [&](int64_t k, int buf) {
+      if (k < k_end) a.load(k, k_end, lds_at + (uint32_t)(buf * kStage));
+    };
+    auto load_b = [&](int64_t k, int buf) {
+      if (k < k_end) b.load(k, k_end, lds_at + (uint32_t)(buf * kStage + A::kBytes));
+    };
+    for (int s = 0; s < STAGES - 1; ++s) {
+      load_a(k_begin + s * kStep, s);
+      load_b(k_begin + s * kStep, s);
+    }
+    wait_and_meet<0>();
+    read(0, 0, 0);
+    int buf = 0;
+    for (int64_t k = k_begin; k < k_end; k += kStep) {
+      const int next = buf + 1 == STAGES ? 0 : buf + 1, last = buf == 0 ? STAGES - 1 : buf - 1;
+      const int64_t k_last = k + (STAGES - 1) * kStep;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) fb[j] = B::fragment(cur + A::kBytes, wn + j * 32, part);
+      for (int part = 0; part < kParts; ++part) {
+        const int set = part & 1;
+        if (part == 0) load_a(k_last, last);
+        if (part < kParts - 1) {
+          read(buf, part + 1, set ^ 1);
+        } else {
+          if (k_last < k_end)
+            wait_and_meet<(STAGES - 3) * (A::kLoads + B::kLoads) + A::kLoads>();
+          else
+            wait_and_meet<0>();
+          read(next, 0, 0);
+          load_b(k_last, last);
+        }
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-          for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(fa[i], fb[j], acc[i][j]);
+          for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(fa[set][i], fb[set][j], acc[i][j]);
       }
+      buf = next;
     }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    wait_and_meet<0>();
   }
 
   // The tile as rows of n (row n: BM values of m) in LDS, chunk c of row n in

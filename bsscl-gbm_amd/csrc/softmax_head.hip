@@ -180,6 +180,14 @@ __device__ __forceinline__ TileAt tile_at(uint32_t at, uint32_t slow, uint32_t f
   return {(int32_t)(in / width), (int32_t)(group * kGroup + in % width)};
 }
 
+// tanh(s / c) for to_exp = 2 log2(e) / c, off by less than 2.5 of 2^-24: as
+// 1 - 2 / (1 + e^{2 |s| / c}) the quotient is at most 1 and the exponential's
+// error counts at most half.
+__device__ __forceinline__ float tanh_of(float s, float to_exp) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(s) * to_exp);
+  return copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e), s);
+}
+
 // Score tiles: BM classes x BN rows.
 template <typename TL>
 __global__ __launch_bounds__(TL::kThreads) void k_scores(
@@ -204,51 +212,72 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
 
   const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
   const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
-  // A lane holds rows wn + 32 j + l % 32 and every fourth group of four
-  // classes; lanes l and l + 32 and the waves along m share a row.
+  // Everything up to the exponential is one instruction a score where it can
+  // be: caps, classes beyond the vocabulary and labels are looked after by
+  // branches that all lanes of a wave take together.
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          acc[i][j][r] = f(acc[i][j][r], wm + i * 32 + (r >> 2) * 8 + (l >> 5) * 4 + (r & 3));
+  };
+  if (softcap > 0.f) {
+    const float to_exp = 2.f * kLog2E / softcap;
+    each([&](float z, int) { return softcap * tanh_of(z, to_exp); });
+  }
+  if (v0 + TL::BM > vocab)
+    each([&](float z, int v) { return v0 + v < vocab ? z : -INFINITY; });
+  // A lane holds rows wn + 32 j + l % 32 and every other group of four classes;
+  // lanes l and l + 32 and the waves along m share a row.
   float *part = reinterpret_cast<float *>(lds);  // [kWavesM][BN]
   float top[TL::NI];
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
     const int n = wn + j * 32 + (l & 31);
-    const int32_t y = r0 + n < pc.rows ? lab[pc.begin + r0 + n] - v0 : -1;
+    const int32_t y = (r0 + n < pc.rows ? lab[pc.begin + r0 + n] - v0 : -1) - wm;
+    if (__any(y >= 0 && y < TL::WM)) {
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (i * 32 + (r >> 2) * 8 + (l >> 5) * 4 + (r & 3) == y) z_label[r0 + n] = acc[i][j][r];
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int v = wm + i * 32 + (r >> 2) * 8 + (l >> 5) * 4 + (r & 3);
-        float z = acc[i][j][r];
-        if (softcap > 0.f) z = softcap * tanhf(z / softcap);
-        z = v0 + v < vocab ? z : -INFINITY;
-        if (v == y) z_label[r0 + n] = z;
-        acc[i][j][r] = z;
-        m = fmaxf(m, z);
-      }
-    m = fmaxf(m, __shfl_xor(m, 32));
-    if (l < 32) part[wave / TL::kWavesN * TL::BN + n] = m;
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+    top[j] = fmaxf(m, __shfl_xor(m, 32));
+    if (TL::kWavesM > 1 && l < 32) part[wave / TL::kWavesN * TL::BN + n] = top[j];
   }
-  __syncthreads();
+  if constexpr (TL::kWavesM > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < TL::NI; ++j)
+#pragma unroll
+      for (int w = 0; w < TL::kWavesM; ++w)
+        top[j] = fmaxf(top[j], part[w * TL::BN + wn + j * 32 + (l & 31)]);
+    __syncthreads();
+  }
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
-    float m = part[wn + j * 32 + (l & 31)];
-    for (int w = 1; w < TL::kWavesM; ++w) m = fmaxf(m, part[w * TL::BN + wn + j * 32 + (l & 31)]);
-    top[j] = m;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < TL::NI; ++j) {
-    const float base = top[j] == -INFINITY ? 0.f : top[j];
+    const float base = top[j] == -INFINITY ? 0.f : -top[j] * kLog2E;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float z = acc[i][j][r], e = __builtin_amdgcn_exp2f((z - base) * kLog2E);
+        const float z = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(z, kLog2E, base));
         s += e;
-        if (P) {
-          const float t = softcap > 0.f && e > 0.f ? z / softcap : 0.f;
-          acc[i][j][r] = e * (1.f - t * t) * kExpScale<T>;
+        if (!P) continue;
+        if (softcap > 0.f) {
+          const float t = e > 0.f ? z / softcap : 0.f;
+          acc[i][j][r] = e * (kExpScale<T> - kExpScale<T> * t * t);
+        } else {
+          acc[i][j][r] = e * kExpScale<T>;
         }
       }
     s += __shfl_xor(s, 32);
@@ -538,9 +567,9 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const HeadInfo *info, const i
 enum Shape : int32_t { kBig, kMid, kThin };
 template <typename T, Shape S, bool A_ACROSS, bool B_ACROSS>
 using TileOf = std::conditional_t<
-    S == kBig, Tile<T, 256, 256, 128, 64, A_ACROSS, B_ACROSS>,
-    std::conditional_t<S == kMid, Tile<T, 128, 128, 64, 64, A_ACROSS, B_ACROSS>,
-                       Tile<T, 128, 32, 32, 32, A_ACROSS, B_ACROSS>>>;
+    S == kBig, Tile<T, 256, 256, 128, 64, A_ACROSS, B_ACROSS, 64, 4>,
+    std::conditional_t<S == kMid, Tile<T, 128, 128, 64, 64, A_ACROSS, B_ACROSS, 64, 4>,
+                       Tile<T, 128, 32, 32, 32, A_ACROSS, B_ACROSS, 128, 3>>>;
 constexpr int shape_m(Shape s) { return s == kBig ? 256 : 128; }
 constexpr int shape_n(Shape s) { return s == kBig ? 256 : s == kMid ? 128 : 32; }
 
@@ -593,7 +622,7 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
     // (four rounds of them, so that the last one weighs little), each of at
     // least 16 steps.
     p.d_hidden = piece <= 32 ? kThin : !f32 && width >= 256 && piece >= 256 ? kBig : kMid;
-    const int64_t step = kStepBytes / es, steps = (vocab + step - 1) / step;
+    const int64_t step = 128 / es, steps = (vocab + step - 1) / step;
     const int64_t want = (4 * kCus + tiles_of(p.d_hidden, width, piece) - 1) /
                          tiles_of(p.d_hidden, width, piece);
     const int64_t splits = std::max<int64_t>(1, std::min(want, steps / 16));
