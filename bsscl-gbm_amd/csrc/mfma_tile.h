@@ -121,26 +121,34 @@ struct Operand {
     }
   }
 
-  // The step that begins at k of k_end, into LDS at lds_at.
-  __device__ __forceinline__ void load(int64_t k, int64_t k_end, uint32_t lds_at) const {
+  // The step that begins at k of k_end, into LDS at lds_at: its buffer
+  // descriptor, and the wave's loads one by one.
+  struct Step {
+    Int4 rsrc;
+    uint32_t at;
+    int32_t bytes;
+  };
+  __device__ __forceinline__ Step step(int64_t k, int64_t k_end, uint32_t lds_at) const {
     const int64_t left = k_end - k;
-    const uint32_t at = lds_at + ((uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) << 10);
+    Step s;
+    s.at = lds_at + ((uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) << 10);
     if constexpr (!ACROSS) {
       // (Rows are padded to whole chunks.)
-      const int32_t bytes = (int32_t)min((left * kES + 15) & ~int64_t(15), (int64_t)STEP);
-      const Int4 r = buffer_of(base + k * kES,
-                               valid > 0 ? (uint32_t)((valid - 1) * stride) + (uint32_t)bytes : 0);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        load_to_lds(r, (int)(chunk * 16) < bytes ? offset[i] : kNoRead, at + i * WAVES * 1024);
+      s.bytes = (int32_t)min((left * kES + 15) & ~int64_t(15), (int64_t)STEP);
+      s.rsrc = buffer_of(base + k * kES,
+                         valid > 0 ? (uint32_t)((valid - 1) * stride) + (uint32_t)s.bytes : 0);
     } else {
       const int32_t rows = (int32_t)min(left, (int64_t)kStep);
-      const Int4 r = buffer_of(base + k * stride,
-                               valid > 0 ? (uint32_t)((rows - 1) * stride) + (uint32_t)(valid * kES)
-                                         : 0);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) load_to_lds(r, offset[i], at + i * WAVES * 1024);
+      s.bytes = STEP;
+      s.rsrc = buffer_of(base + k * stride, valid > 0 ? (uint32_t)((rows - 1) * stride) +
+                                                            (uint32_t)(valid * kES)
+                                                      : 0);
     }
+    return s;
+  }
+  __device__ __forceinline__ void load(const Step &s, int i) const {
+    const bool in = ACROSS || (int)(chunk * 16) < s.bytes;
+    load_to_lds(s.rsrc, in ? offset[i] : kNoRead, s.at + (uint32_t)(i * WAVES * 1024));
   }
 
   // The fragment of k part `part` (of STEP / 32) and the 32 rows from `first` on.
@@ -194,64 +202,84 @@ struct Tile {
   // acc[mi][ni] += products of k in [k_begin, k_end); k_begin is a multiple of
   // kStep.  Every thread of the workgroup calls it; LDS is free at its end.
   //
-  // Step k is read while those up to k + STAGES - 1 load: A's part of the last
-  // one is issued at the step's beginning, B's in its last part (all at once,
-  // every wave would wait for the address units while the matrix cores idle).
-  // Fragments are read one part ahead of the products that use them, the first
-  // part of a step during the last products of the step before: there stands
-  // the step's one barrier, when every wave has read the last of its buffer
-  // and the next step's own loads have landed.
+  // Step k is read while those up to k + STAGES - 1 load.  Fragments are read
+  // one part ahead of the products that use them, the first part of a step
+  // during the last products of the step before: there stands the step's one
+  // barrier, when every wave has read the last of its buffer and the next
+  // step's loads have landed.  Reads and loads are dealt out among the
+  // products (A's loads to the first part, B's to the last), so that no more
+  // than a few are issued between two of them: the matrix cores multiply on
+  // meanwhile.
   __device__ static __forceinline__ void walk(const A &a, const B &b, int64_t k_begin,
                                               int64_t k_end, char *lds, Acc16 (&acc)[MI][NI]) {
     const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / kWavesN * WM, wn = wave % kWavesN * WN;
     const uint32_t lds_at =
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    constexpr int kReads = MI + NI;
     Int4 fa[2][MI], fb[2][NI];
-    auto read = [&](int buf, int part, int set) {
-      const char *cur = lds + buf * kStage;
-#pragma unroll
-      for (int j = 0; j < NI; ++j) fb[set][j] = B::fragment(cur + A::kBytes, wn + j * 32, part);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) fa[set][i] = A::fragment(cur, wm + i * 32, part);
-    };
-    auto load_a = [&](int64_t k, int buf) {
-      if (k < k_end) a.load(k, k_end, lds_at + (uint32_t)(buf * kStage));
-    };
-    auto load_b = [&](int64_t k, int buf) {
-      if (k < k_end) b.load(k, k_end, lds_at + (uint32_t)(buf * kStage + A::kBytes));
+    auto read = [&](const char *cur, int part, int set, int i) {
+      if (i < NI)
+        fb[set][i] = B::fragment(cur + A::kBytes, wn + i * 32, part);
+      else
+        fa[set][i - NI] = A::fragment(cur, wm + (i - NI) * 32, part);
     };
     for (int s = 0; s < STAGES - 1; ++s) {
-      load_a(k_begin + s * kStep, s);
-      load_b(k_begin + s * kStep, s);
+      const int64_t k = k_begin + s * kStep;
+      if (k >= k_end) break;
+      const auto sa = a.step(k, k_end, lds_at + (uint32_t)(s * kStage));
+      const auto sb = b.step(k, k_end, lds_at + (uint32_t)(s * kStage + A::kBytes));
+#pragma unroll
+      for (int i = 0; i < A::kLoads; ++i) a.load(sa, i);
+#pragma unroll
+      for (int i = 0; i < B::kLoads; ++i) b.load(sb, i);
     }
     wait_and_meet<0>();
-    read(0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) read(lds, 0, 0, i);
     int buf = 0;
-    for (int64_t k = k_begin; k < k_end; k += kStep) {
-      const int next = buf + 1 == STAGES ? 0 : buf + 1, last = buf == 0 ? STAGES - 1 : buf - 1;
-      const int64_t k_last = k + (STAGES - 1) * kStep;
+    // MORE: there is a step to load.
+    auto one_step = [&](int64_t k, auto more) {
+      constexpr bool MORE = decltype(more)::value;
+      const int next = buf + 1 == STAGES ? 0 : buf + 1;
+      const char *cur = lds + buf * kStage, *then = lds + next * kStage;
+      typename A::Step sa;
+      typename B::Step sb;
+      if constexpr (MORE) {
+        const uint32_t at = lds_at + (uint32_t)((buf == 0 ? STAGES - 1 : buf - 1) * kStage);
+        sa = a.step(k + (STAGES - 1) * kStep, k_end, at);
+        sb = b.step(k + (STAGES - 1) * kStep, k_end, at + A::kBytes);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
         const int set = part & 1;
-        if (part == 0) load_a(k_last, last);
-        if (part < kParts - 1) {
-          read(buf, part + 1, set ^ 1);
-        } else {
-          if (k_last < k_end)
-            wait_and_meet<(STAGES - 3) * (A::kLoads + B::kLoads) + A::kLoads>();
-          else
-            wait_and_meet<0>();
-          read(next, 0, 0);
-          load_b(k_last, last);
-        }
+        if (part == kParts - 1)
+          wait_and_meet<MORE ? (STAGES - 3) * (A::kLoads + B::kLoads) + A::kLoads : 0>();
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i) {
+          if constexpr (MORE) {
+            if (part == 0)
+#pragma unroll
+              for (int e = i * A::kLoads / MI; e < (i + 1) * A::kLoads / MI; ++e) a.load(sa, e);
+            if (part == kParts - 1)
+#pragma unroll
+              for (int e = i * B::kLoads / MI; e < (i + 1) * B::kLoads / MI; ++e) b.load(sb, e);
+          }
+#pragma unroll
+          for (int e = i * kReads / MI; e < (i + 1) * kReads / MI; ++e)
+            read(part < kParts - 1 ? cur : then, part < kParts - 1 ? part + 1 : 0, set ^ 1, e);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(fa[set][i], fb[set][j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       buf = next;
-    }
+    };
+    int64_t k = k_begin;
+    for (; k + (STAGES - 1) * kStep < k_end; k += kStep) one_step(k, std::true_type());
+    for (; k < k_end; k += kStep) one_step(k, std::false_type());
     wait_and_meet<0>();
   }
 

@@ -613,8 +613,14 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
   p.tiles = (int32_t)((vocab + p.tile_v - 1) / p.tile_v);
   p.ldp = (int64_t)p.tiles * p.tile_v;
   const int64_t row_bytes = grad ? p.ldp * es : (int64_t)p.tiles * (int64_t)sizeof(float2);
-  const int64_t fit = std::max<int64_t>(kRowPad, kPieceBytes / row_bytes / kRowPad * kRowPad);
-  p.piece_rows = (int32_t)std::min<int64_t>(fit, round_up(rows, kRowPad));
+  // One piece takes no float32 sums of d_weight: it may have their room.
+  const int64_t one = grad ? kPieceBytes + vocab * p.wide * 4 : kPieceBytes;
+  const int64_t all = round_up(rows, kRowPad);
+  const int64_t fit =
+      all * row_bytes <= one
+          ? all
+          : std::max<int64_t>(kRowPad, kPieceBytes / row_bytes / kRowPad * kRowPad);
+  p.piece_rows = (int32_t)std::min<int64_t>(fit, all);
   p.pieces = (int32_t)((rows + p.piece_rows - 1) / p.piece_rows);
   if (grad) {
     const int64_t piece = std::min<int64_t>(rows, p.piece_rows);
