@@ -317,6 +317,15 @@ struct Tile {
                                         ((c ^ (n & (kOutChunks - 1))) << 4)));
     }
   }
+  // f(n, m, value) for the values of this thread, neighbours side by side.
+  template <typename F>
+  __device__ static __forceinline__ void read_out_one(const char *lds, F &&f) {
+    for (int e = (int)threadIdx.x; e < BN * BM; e += kThreads) {
+      const int n = e / BM, m = e % BM, at = m * (int)sizeof(T);
+      const int c = (at >> 4) ^ (n & (kOutChunks - 1));
+      f(n, m, *reinterpret_cast<const T *>(lds + n * kOutRow + (c << 4) + (at & 15)));
+    }
+  }
 };
 
 // Workgroup b of `count` in an order that gives each of the 8 XCDs (which take

@@ -188,16 +188,19 @@ __device__ __forceinline__ float tanh_of(float s, float to_exp) {
   return copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e), s);
 }
 
-// Score tiles: BM classes x BN rows.
-template <typename TL>
+// Score tiles: BM classes x BN rows.  Label: int32 for packed rows, int64 for
+// rows as the caller has them (info: none; `piece` rows).
+template <typename TL, typename Label>
 __global__ __launch_bounds__(TL::kThreads) void k_scores(
     const typename TL::T *weight, int64_t w_stride, int32_t vocab, int32_t width,
-    const typename TL::T *packed, int32_t wide, const int32_t *lab, const HeadInfo *info,
+    const typename TL::T *packed, int64_t wide, const Label *lab, const HeadInfo *info,
     int32_t piece, int32_t pieces, float softcap, int32_t tiles, float2 *stats, float *z_label,
     typename TL::T *P, int64_t ldp) {
   using T = typename TL::T;
   __shared__ __align__(1024) char lds[TL::kLdsOut];
-  const Piece pc = piece_of(info->rows, piece, pieces);
+  constexpr bool kPacked = sizeof(Label) == 4;
+  Piece pc{0, piece};
+  if constexpr (kPacked) pc = piece_of(info->rows, piece, pieces);
   const uint32_t row_tiles = (uint32_t)(pc.rows + TL::BN - 1) / TL::BN;
   const uint32_t total = row_tiles * (uint32_t)tiles;
   if (blockIdx.x >= total) return;
@@ -206,7 +209,8 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
   typename TL::A a;
   typename TL::B b;
   a.init(weight, w_stride, v0, vocab);
-  b.init(packed + (int64_t)pc.begin * wide, wide, r0, (pc.rows + kRowPad - 1) / kRowPad * kRowPad);
+  b.init(packed + pc.begin * wide, wide, r0,
+         kPacked ? (pc.rows + kRowPad - 1) / kRowPad * kRowPad : pc.rows);
   Acc16 acc[TL::MI][TL::NI] = {};
   TL::walk(a, b, 0, width, lds, acc);
 
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
     const int n = wn + j * 32 + (l & 31);
-    const int32_t y = (r0 + n < pc.rows ? lab[pc.begin + r0 + n] - v0 : -1) - wm;
+    const Label y = (r0 + n < pc.rows ? lab[pc.begin + r0 + n] : -1) - v0 - wm;
     if (__any(y >= 0 && y < TL::WM)) {
 #pragma unroll
       for (int i = 0; i < TL::MI; ++i)
@@ -312,24 +316,32 @@ __device__ __forceinline__ float wave_add(float v) {
   return v;
 }
 
+// (m, s) with s exp(m) the sum over the tiles first, first + by, ...: rescaled
+// as the maximum grows.
+__device__ __forceinline__ float2 tiles_sum(const float2 *st, int32_t tiles, int32_t first,
+                                            int32_t by) {
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 4
+  for (int32_t t = first; t < tiles; t += by) {
+    const float2 x = st[t];
+    if (x.x > m) {
+      s = m == -INFINITY ? x.y : s * expf(m - x.x) + x.y;
+      m = x.x;
+    } else {
+      s += x.x == -INFINITY ? x.y : x.y * expf(x.x - m);  // (NaN stays NaN)
+    }
+  }
+  return make_float2(m, s);
+}
+
 // lse of a row from its tiles' statistics, by the block's kRowThreads threads.
 constexpr int kRowThreads = 256;
 __device__ float row_lse(const float2 *st, int32_t tiles, float *red) {
   constexpr int kWaves = kRowThreads / 64;
   const int tid = (int)threadIdx.x, wid = tid >> 6;
-  // Each thread's own maximum and sum first, rescaled as the maximum grows.
-  float m = -INFINITY, s = 0.f;
-  for (int t = tid; t < tiles; t += kRowThreads) {
-    const float2 x = st[t];
-    if (x.x > m) {
-      s = m == -INFINITY ? x.y : s * expf(m - x.x) + x.y;
-      m = x.x;
-    } else if (x.x != -INFINITY) {
-      s += x.y * expf(x.x - m);
-    } else {
-      s += x.y;  // NaN stays NaN
-    }
-  }
+  const float2 own = tiles_sum(st, tiles, tid, kRowThreads);
+  const float m = own.x;
+  float s = own.y;
   float top = wave_max(m);
   if ((tid & 63) == 0) red[wid] = top;
   __syncthreads();
@@ -343,6 +355,49 @@ __device__ float row_lse(const float2 *st, int32_t tiles, float *red) {
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) s += red[kWaves + w];
   return (top == -INFINITY ? 0.f : top) + logf(s);
+}
+
+// Up to kFewRows rows as the caller has them, one block: each wave takes a part
+// of a row's tiles, and the rows' weighted sum follows in their order.
+constexpr int kFewRows = 32;
+__global__ __launch_bounds__(1024) void k_few_rows(const int64_t *labels, const float *row_weight,
+                                                   int32_t rows, int32_t vocab, int32_t mean,
+                                                   float z_loss, int32_t tiles,
+                                                   const float2 *stats, const float *z_label,
+                                                   float *loss, float *row_loss, float *lse_out) {
+  constexpr int kWaves = 16;
+  __shared__ float2 part[kFewRows][kWaves];
+  __shared__ float value[kFewRows];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  const int parts = rows <= 1 ? 16 : rows <= 2 ? 8 : rows <= 4 ? 4 : rows <= 8 ? 2 : 1;
+  for (int r = wave / parts; r < rows; r += kWaves / parts) {
+    float2 x = tiles_sum(stats + (int64_t)r * tiles, tiles, wave % parts * 64 + lane, parts * 64);
+    const float top = wave_max(x.x);
+    x.y = wave_add(x.x == -INFINITY ? x.y : x.y * expf(x.x - top));
+    if (lane == 0) part[r][wave % parts] = make_float2(top, x.y);
+  }
+  __syncthreads();
+  const int r = (int)threadIdx.x;
+  if (r < rows) {
+    const float2 x = tiles_sum(part[r], parts, 0, 1);
+    const float lse = (x.x == -INFINITY ? 0.f : x.x) + logf(x.y);
+    const int64_t y = labels[r];
+    const bool counts = y >= 0 && y < vocab;
+    const float l = counts ? lse - z_label[r] + z_loss * lse * lse : 0.f;
+    row_loss[r] = l;
+    lse_out[r] = counts ? lse : 0.f;
+    value[r] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  double s = 0.0, all = 0.0;
+  for (int i = 0; i < rows; ++i) {
+    if (labels[i] < 0 || labels[i] >= vocab) continue;
+    const double w = row_weight ? row_weight[i] : 1.0;
+    all += w;
+    s += w * value[i];
+  }
+  *loss = (float)(!mean ? s : all != 0.0 ? s / all : 0.0);
 }
 
 // One block per row of the piece: lse and loss from the tiles' statistics;
@@ -458,17 +513,29 @@ __global__ __launch_bounds__(256) void k_d_hidden_sum(const HeadInfo *info, int3
                                                       int32_t splits, const float *part,
                                                       int64_t part_stride, int32_t wide,
                                                       int32_t width, T *d_hidden,
-                                                      int64_t d_stride) {
+                                                      int64_t d_stride, int32_t vec) {
   const Piece pc = piece_of(info->rows, piece, pieces);
   const int32_t r = (int32_t)blockIdx.x;
   if (r >= pc.rows) return;
   const float back = info->from_operand;
-  T *out = d_hidden + (int64_t)idx[pc.begin + r] * d_stride;
-  for (int32_t d = (int32_t)threadIdx.x; d < width; d += 256) {
+  T *row = d_hidden + (int64_t)idx[pc.begin + r] * d_stride;
+  for (int32_t d = (int32_t)threadIdx.x * 4; d < width; d += 1024) {
     const float *p = part + (int64_t)r * wide + d;
-    float s = 0.f;
-    for (int32_t k = 0; k < splits; ++k) s += p[(int64_t)k * part_stride];
-    out[d] = (T)(s * back);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int32_t k = 0; k < splits; ++k) {
+      const float4 x = *reinterpret_cast<const float4 *>(p + (int64_t)k * part_stride);
+      s = make_float4(s.x + x.x, s.y + x.y, s.z + x.z, s.w + x.w);
+    }
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T4 v = {(T)(s.x * back), (T)(s.y * back), (T)(s.z * back), (T)(s.w * back)};
+    if (vec && d + 4 <= width) {
+      *reinterpret_cast<T4 *>(row + d) = v;
+      continue;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < width) row[d + e] = v[e];
   }
 }
 
@@ -524,29 +591,37 @@ __global__ __launch_bounds__(TL::kThreads) void k_d_weight(
   const float back = info->from_operand;
   TL::stage_out(lds, [&](int i, int j, int r) { return (T)(acc[i][j][r] * back); });
   __syncthreads();
-  TL::read_out(lds, [&](int n, int m, Int4 x) {
-    if (v0 + n >= vocab) return;
-    T *out = d_weight + (int64_t)(v0 + n) * d_stride + d0 + m;
-    constexpr int kVec = 16 / (int)sizeof(T);
-    if (vec && d0 + m + kVec <= width) {
-      *reinterpret_cast<Int4 *>(out) = x;
-      return;
-    }
-    T e[kVec];
-    __builtin_memcpy(e, &x, 16);
-#pragma unroll
-    for (int k = 0; k < kVec; ++k)
-      if (d0 + m + k < width) out[k] = e[k];
-  });
+  if (vec) {
+    TL::read_out(lds, [&](int n, int m, Int4 x) {
+      if (v0 + n < vocab && d0 + m < width)
+        *reinterpret_cast<Int4 *>(d_weight + (int64_t)(v0 + n) * d_stride + d0 + m) = x;
+    });
+  } else {
+    TL::read_out_one(lds, [&](int n, int m, T x) {
+      if (v0 + n < vocab && d0 + m < width) d_weight[(int64_t)(v0 + n) * d_stride + d0 + m] = x;
+    });
+  }
 }
 
-// Rows of the weight at a stride and width that the tiles can load from.
+// Rows of the weight at a stride and width that the tiles can load from: a
+// thread gathers 16 bytes of a row.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack_weight(const T *weight, int64_t stride,
-                                                     int32_t width, int32_t wide, T *packed) {
-  const int64_t v = (int64_t)blockIdx.x;
-  for (int32_t d = (int32_t)threadIdx.x; d < wide; d += 256)
-    packed[v * wide + d] = d < width ? weight[v * stride + d] : (T)0.f;
+                                                     int32_t vocab, int32_t width, int32_t wide,
+                                                     T *packed) {
+  constexpr int N = 16 / (int)sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(N)));
+  const uint32_t chunks = (uint32_t)wide / N;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;; e += (int64_t)gridDim.x * 256) {
+    const int64_t v = e / chunks;
+    if (v >= vocab) return;
+    const int32_t d = (int32_t)(e - v * chunks) * N;
+    const T *from = weight + v * stride + d;
+    TV x;
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = d + k < width ? from[k] : (T)0.f;
+    *reinterpret_cast<TV *>(packed + e * N) = x;
+  }
 }
 
 // loss = sum of u * row_loss over the counting rows, in their order.
@@ -589,13 +664,18 @@ struct HeadPlan {
   size_t info, idx, lab, u, pos, packed, stats, z_label, P, part, sum, weight, bytes;
 };
 
+// Grids stay below 2^32 threads, and what a tile loads within 2^31 bytes.
+constexpr int64_t kMostRows = 8000000, kMostVocab = 4000000, kMostWidth = 65536;
+constexpr int64_t kMostPiece = 1 << 20;
+
 int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const void *weight,
               int64_t w_stride, bool grad, HeadPlan *pl) {
   if (dtype != BSSCL_BF16 && dtype != BSSCL_F16 && dtype != BSSCL_F32)
     return set_error(BSSCL_EINVAL, "softmax head: unknown dtype " + std::to_string(dtype));
-  if (rows < 1 || vocab < 1 || width < 1 || rows >= (1 << 30) || vocab > 4000000 || width > 65536)
+  if (rows < 1 || vocab < 1 || width < 1 || rows > kMostRows || vocab > kMostVocab ||
+      width > kMostWidth)
     return set_error(BSSCL_EINVAL,
-                     "softmax head: rows must be in [1, 2^30), vocab in [1, 4000000], width in "
+                     "softmax head: rows must be in [1, 8000000], vocab in [1, 4000000], width in "
                      "[1, 65536]");
   const bool f32 = dtype == BSSCL_F32;
   const int64_t es = f32 ? 4 : 2;
@@ -604,9 +684,11 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
   p.width = (int32_t)width;
   p.wide = (int32_t)round_up(width, kColPad);
   p.vocab = (int32_t)vocab;
+  // The largest tile that gives every CU one; few rows or classes take the
+  // smallest.
   auto shape = [&](int64_t m, int64_t n) {
-    if (n <= 32) return kThin;
-    return !f32 && tiles_of(kBig, m, n) >= kCus ? kBig : kMid;
+    if (!f32 && tiles_of(kBig, m, n) >= kCus) return kBig;
+    return n > 32 && tiles_of(kMid, m, n) >= kCus ? kMid : kThin;
   };
   p.scores = shape(vocab, rows);
   p.tile_v = shape_m(p.scores);
@@ -617,22 +699,35 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
   const int64_t one = grad ? kPieceBytes + vocab * p.wide * 4 : kPieceBytes;
   const int64_t all = round_up(rows, kRowPad);
   const int64_t fit =
-      all * row_bytes <= one
+      all * row_bytes <= one && all <= kMostPiece
           ? all
           : std::max<int64_t>(kRowPad, kPieceBytes / row_bytes / kRowPad * kRowPad);
-  p.piece_rows = (int32_t)std::min<int64_t>(fit, all);
+  p.piece_rows = (int32_t)std::min({fit, all, kMostPiece});
   p.pieces = (int32_t)((rows + p.piece_rows - 1) / p.piece_rows);
   if (grad) {
     const int64_t piece = std::min<int64_t>(rows, p.piece_rows);
-    // d_hidden's sums run over the whole vocabulary: parts of it fill the CUs
-    // (four rounds of them, so that the last one weighs little), each of at
-    // least 16 steps.
     p.d_hidden = piece <= 32 ? kThin : !f32 && width >= 256 && piece >= 256 ? kBig : kMid;
+    if (p.d_hidden == kMid && tiles_of(kMid, width, piece) < kCus / 16) p.d_hidden = kThin;
+    // d_hidden's sums run over the whole vocabulary, in parts that fill the
+    // CUs.  What a number of parts costs, in microseconds: rounds of tiles (a
+    // CU holds one kBig, two kMid or kThin), each with a start and an end, and
+    // the parts' sums written and read.  The rates are the kernels' own.
     const int64_t step = 128 / es, steps = (vocab + step - 1) / step;
-    const int64_t want = (4 * kCus + tiles_of(p.d_hidden, width, piece) - 1) /
-                         tiles_of(p.d_hidden, width, piece);
-    const int64_t splits = std::max<int64_t>(1, std::min(want, steps / 16));
-    p.split_v = (int32_t)((steps + splits - 1) / splits * step);
+    const int64_t tiles = tiles_of(p.d_hidden, width, piece);
+    const int64_t at_once = p.d_hidden == kBig ? kCus : 2 * kCus;
+    const double step_us = (f32 ? 8.0 : 1.0) * (p.d_hidden == kBig ? 1.4 : p.d_hidden == kMid ? 0.8 : 0.3);
+    const double part_us = (double)piece * p.wide * 8 / 4e6;
+    double best = 0.0;
+    for (int64_t n = 1; n <= std::min<int64_t>(64, std::max<int64_t>(1, steps / 4)); ++n) {
+      const double us = (double)((tiles * n + at_once - 1) / at_once) *
+                            ((double)((steps + n - 1) / n) * step_us + 6.0) +
+                        (double)n * part_us;
+      if (n == 1 || us < best) {
+        best = us;
+        p.splits = (int32_t)n;
+      }
+    }
+    p.split_v = (int32_t)((steps + p.splits - 1) / p.splits * step);
     p.splits = (int32_t)((vocab + p.split_v - 1) / p.split_v);
     p.d_weight = !f32 && tiles_of(kBig, width, vocab) >= kCus ? kBig : kMid;
   }
@@ -686,6 +781,12 @@ void by_shape(Shape s, F &&f) {
   f(std::integral_constant<Shape, kMid>());
 }
 
+int launched() {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return BSSCL_OK;
+  return set_error(BSSCL_EDEVICE, std::string("softmax head: ") + hipGetErrorString(e));
+}
+
 template <typename T>
 int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
   auto *info = reinterpret_cast<HeadInfo *>(c.ws + p.info);
@@ -702,9 +803,25 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
   auto *weight = static_cast<const T *>(c.weight);
   int64_t w_stride = c.w_stride;
   int32_t w_width = p.width;
+  constexpr int64_t kSize = (int64_t)sizeof(T);
+  // A few rows to be scored, where the tiles can load them: two launches.
+  if (!c.grad && p.rows <= kFewRows && !p.pack_weight && ((uintptr_t)c.hidden & 15) == 0 &&
+      (p.rows == 1 || (c.h_stride * kSize % 16 == 0 &&
+                       c.h_stride * kSize * kFewRows < (int64_t(1) << 31)))) {
+    using TL = TileOf<T, kThin, false, false>;
+    k_scores<TL, int64_t><<<(unsigned)p.tiles, TL::kThreads, 0, st>>>(
+        weight, w_stride, p.vocab, p.width, static_cast<const T *>(c.hidden),
+        p.rows == 1 ? p.width : c.h_stride, c.labels, nullptr, p.rows, 1, c.softcap, p.tiles, stats,
+        z_label, nullptr, 0);
+    k_few_rows<<<1, 1024, 0, st>>>(c.labels, c.row_weight, p.rows, p.vocab, c.mean, c.z_loss,
+                                   p.tiles, stats, z_label, c.loss, c.row_loss, c.lse);
+    return launched();
+  }
   if (p.pack_weight) {
     auto *w = reinterpret_cast<T *>(c.ws + p.weight);
-    k_pack_weight<T><<<(unsigned)p.vocab, 256, 0, st>>>(weight, w_stride, p.width, p.wide, w);
+    const int64_t chunks = (int64_t)p.vocab * p.wide * (int64_t)sizeof(T) / 16;
+    k_pack_weight<T><<<(unsigned)std::min<int64_t>((chunks + 255) / 256, 1 << 20), 256, 0, st>>>(
+        weight, w_stride, p.vocab, p.width, p.wide, w);
     weight = w;
     w_stride = w_width = p.wide;
   }
@@ -716,11 +833,14 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
       static_cast<T *>(c.d_hidden), c.dh_stride);
   const int64_t piece = std::min<int64_t>(p.rows, p.piece_rows);
   const int64_t part_stride = (int64_t)p.piece_rows * p.wide;
-  const int vec = ((uintptr_t)c.d_weight & 15) == 0 && c.dw_stride * (int64_t)sizeof(T) % 16 == 0;
+  const int dw_vec = ((uintptr_t)c.d_weight & 15) == 0 && c.dw_stride * kSize % 16 == 0 &&
+                     p.width * kSize % 16 == 0;
+  const int dh_vec =
+      (uintptr_t)c.d_hidden % (4 * sizeof(T)) == 0 && c.dh_stride % 4 == 0;
   for (int32_t k = 0; k < p.pieces; ++k) {
     by_shape<T, true>(p.scores, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, false, false>;
-      k_scores<TL><<<(unsigned)tiles_of(s, p.vocab, piece), TL::kThreads, 0, st>>>(
+      k_scores<TL, int32_t><<<(unsigned)tiles_of(s, p.vocab, piece), TL::kThreads, 0, st>>>(
           weight, w_stride, p.vocab, w_width, packed, p.wide, lab, info, k, p.pieces, c.softcap,
           p.tiles, stats, z_label, P, p.ldp);
     });
@@ -734,23 +854,20 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
                                                 p.wide, info, k, p.pieces, p.splits, p.split_v,
                                                 part, part_stride);
     });
-    k_d_hidden_sum<T><<<(unsigned)piece, 256, 0, st>>>(info, k, p.pieces, idx, p.splits, part,
-                                                       part_stride, p.wide, p.width,
-                                                       static_cast<T *>(c.d_hidden), c.dh_stride);
+    k_d_hidden_sum<T><<<(unsigned)piece, 256, 0, st>>>(
+        info, k, p.pieces, idx, p.splits, part, part_stride, p.wide, p.width,
+        static_cast<T *>(c.d_hidden), c.dh_stride, dh_vec);
     by_shape<T, false>(p.d_weight, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, true, true>;
       k_d_weight<TL><<<(unsigned)tiles_of(s, p.width, 1) *
                            (unsigned)((p.vocab + TL::BN - 1) / TL::BN),
                        TL::kThreads, 0, st>>>(
           P, p.ldp, packed, p.wide, p.vocab, p.width, info, k, p.pieces, sum,
-          static_cast<T *>(c.d_weight), c.dw_stride, vec);
+          static_cast<T *>(c.d_weight), c.dw_stride, dw_vec);
     });
   }
   k_loss_sum<<<1, 1024, 0, st>>>(info, idx, u, c.row_loss, c.loss);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return set_error(BSSCL_EDEVICE, std::string("softmax head: ") + hipGetErrorString(e));
-  return BSSCL_OK;
+  return launched();
 }
 
 int head(int32_t device, void *stream, int32_t dtype, int64_t rows, int64_t width, int64_t vocab,

@@ -511,7 +511,7 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
  * it has been normalised, as operand of the two products.  In float16 it is
  * scaled by a power of two first (it holds at least 2^-35 of the largest row
  * weight), and 1 + 2 zeta lse may reach 32.
- * 1 <= rows < 2^30, 1 <= width <= 65536, 1 <= vocab <= 4000000.
+ * 1 <= rows <= 8000000, 1 <= width <= 65536, 1 <= vocab <= 4000000.
  */
 int bsscl_head_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t vocab,
                          const void *weight, int64_t weight_stride, int32_t with_grad,

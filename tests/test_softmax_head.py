@@ -81,7 +81,7 @@ def test_c_entries_refuse_bad_sizes():
 
     assert ws(0, 5, 8, 9) == _native.BSSCL_OK and size.value > 0
     for bad in [(3, 5, 8, 9), (-1, 5, 8, 9), (0, 0, 8, 9), (0, 5, 0, 9), (0, 5, 8, 0),
-                (0, 1 << 30, 8, 9), (0, 5, 65537, 9), (0, 5, 8, 4000001)]:
+                (0, 8000001, 8, 9), (0, 5, 65537, 9), (0, 5, 8, 4000001)]:
         assert ws(*bad) == _native.BSSCL_EINVAL
         assert L.bsscl_last_error()
     fake = ctypes.c_void_p(4096)  # never read: every call below is refused on the host
