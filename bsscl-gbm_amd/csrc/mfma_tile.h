@@ -2,24 +2,24 @@
 // bf16, fp16 and float32 operands with float32 sums.
 //
 // A workgroup holds a BM x BN tile in registers, WM x WN per wave in blocks of
-// 32 x 32 (v_mfma 32x32x16, for float32 32x32x2), and walks k in steps.  Both
-// operands' steps go from memory straight to LDS (buffer loads with the lds
-// bit: no registers), into a ring of buffers.  An operand lies in memory with
-// k contiguous (rows of m or n) or with m or n contiguous (rows of k):
+// 16 x 16 (v_mfma 16x16x32, for float32 16x16x4: at the card's power limit they
+// reach 1.9 PFLOP/s in bf16 from registers, 32x32x16 1.7), and walks k in
+// steps.  Both operands' steps go from memory straight to LDS (buffer loads with
+// the lds bit: no registers), into a ring of buffers.  An operand lies in
+// memory with k contiguous (rows of m or n) or with m or n contiguous (rows of
+// k):
 //   k contiguous   LDS rows of one step's bytes; a lane reads 16 bytes of a row
 //   k across rows  LDS rows of the tile's m (n) range; 16-bit fragments come
 //                  from transposing reads (ds_read_b64_tr_b16: a group of 16
-//                  lanes reads 4 k x 16 m and gets k in registers), and chunk
-//                  c of row k lies in place c ^ 4 (k & 3), so that the four
-//                  rows of a group touch different banks
-// An LDS place is lane-linear in the load, so the swizzles permute the lanes'
-// addresses in memory.  Reads outside the operand return 0 (the buffer
-// descriptor's bound), so edges need no other care: offsets of lanes that
-// are not to read are 2^31, beyond every bound.
+//                  lanes reads 4 k x 16 m and gets k in registers)
+// An LDS place is lane-linear in the load, so the places of 16-byte chunks
+// (place_of, which keeps what is read at once on different banks) permute the
+// lanes' addresses in memory.  Reads outside the operand return 0 (the buffer
+// descriptor's bound), so edges need no other care: offsets of lanes that are
+// not to read are 2^31, beyond every bound.
 //
-// Fragment of the 32x32 blocks, lane l: row (column) l % 32 and 16 bytes of k
-// from 16 (l / 32) on; result register r: m = 8 (r / 4) + 4 (l / 32) + r % 4,
-// n = l % 32.
+// Fragment of a 16 x 16 block, lane l: row (column) l % 16 and 16 bytes of k
+// from 16 (l / 16) on; result register r: m = 4 (l / 16) + r, n = l % 16.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -29,7 +29,7 @@
 namespace bsscl {
 
 typedef int Int4 __attribute__((ext_vector_type(4)));
-typedef float Acc16 __attribute__((ext_vector_type(16)));
+typedef float Acc4 __attribute__((ext_vector_type(4)));
 typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 F16x8 __attribute__((ext_vector_type(8)));
 typedef short Short4 __attribute__((ext_vector_type(4)));
@@ -38,17 +38,17 @@ constexpr uint32_t kNoRead = 0x80000000u;  // a lane's offset beyond every bound
 
 // acc += a b over one 16-byte fragment of k.
 template <typename T>
-__device__ __forceinline__ Acc16 mma(Int4 a, Int4 b, Acc16 acc) {
+__device__ __forceinline__ Acc4 mma(Int4 a, Int4 b, Acc4 acc) {
   if constexpr (std::is_same<T, __bf16>::value) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a),
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a),
                                                    __builtin_bit_cast(Bf16x8, b), acc, 0, 0, 0);
   } else if constexpr (std::is_same<T, _Float16>::value) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(F16x8, a),
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(F16x8, a),
                                                   __builtin_bit_cast(F16x8, b), acc, 0, 0, 0);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, (int)a[j]),
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (int)a[j]),
                                                  __builtin_bit_cast(float, (int)b[j]), acc, 0, 0,
                                                  0);
     return acc;
@@ -83,14 +83,20 @@ struct Operand {
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // of each wave in a step
   static_assert(kLoads >= 1 && kLoads * 1024 * WAVES == kBytes && kChunks <= 64, "tile shape");
 
-  // The place of chunk c of LDS row r.  Sixteen lanes read 16 bytes each in one
-  // go: with k contiguous, of one chunk of 16 rows, which lie in all 16
-  // chunks of a bank line (256 bytes: kPerLine rows).
+  // The place of chunk c of LDS row r, its own inverse.  Banks repeat every 256
+  // bytes.  Sixteen lanes read at once
+  //   k contiguous: 16 bytes each, one chunk of 16 rows, kPerLine of which
+  //     share a line of 256 bytes: these rows' places follow from the others';
+  // or 32 lanes
+  //   k across, 16 bits: two chunks of rows k + 0..3 and k + 8..11;
+  //   k across, float32: four chunks of rows k and k + 4 (k + 8, k + 12).
   static constexpr int kPerLine = 256 / kRowBytes > 0 ? 256 / kRowBytes : 1;
   __device__ static __forceinline__ int place_of(int c, int r) {
-    if constexpr (!ACROSS) return c ^ ((r / kPerLine) & (kChunks - 1));
-    else if constexpr (kES == 2) return c ^ (((r & 3) * 4) & (kChunks - 1));
-    else return c;
+    int x;
+    if constexpr (!ACROSS) x = r / kPerLine;
+    else if constexpr (kES == 2) x = (r & 3) * 4 + ((r >> 3) & 1) * 2;
+    else x = ((r >> 2) & 3) * 4;
+    return c ^ (x & (kChunks - 1));
   }
 
   const char *base;
@@ -121,28 +127,28 @@ struct Operand {
     }
   }
 
-  // The step that begins at k of k_end, into LDS at lds_at: its buffer
-  // descriptor, and the wave's loads one by one.
+  // The step that begins at k of k_end (zeros from there on), into LDS at
+  // lds_at: its buffer descriptor, and the wave's loads one by one.
   struct Step {
     Int4 rsrc;
     uint32_t at;
     int32_t bytes;
   };
   __device__ __forceinline__ Step step(int64_t k, int64_t k_end, uint32_t lds_at) const {
-    const int64_t left = k_end - k;
+    const int64_t left = max(k_end - k, (int64_t)0);
+    const bool any = valid > 0 && left > 0;
     Step s;
     s.at = lds_at + ((uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) << 10);
     if constexpr (!ACROSS) {
       // (Rows are padded to whole chunks.)
       s.bytes = (int32_t)min((left * kES + 15) & ~int64_t(15), (int64_t)STEP);
       s.rsrc = buffer_of(base + k * kES,
-                         valid > 0 ? (uint32_t)((valid - 1) * stride) + (uint32_t)s.bytes : 0);
+                         any ? (uint32_t)((valid - 1) * stride) + (uint32_t)s.bytes : 0);
     } else {
       const int32_t rows = (int32_t)min(left, (int64_t)kStep);
       s.bytes = STEP;
-      s.rsrc = buffer_of(base + k * stride, valid > 0 ? (uint32_t)((rows - 1) * stride) +
-                                                            (uint32_t)(valid * kES)
-                                                      : 0);
+      s.rsrc = buffer_of(base + k * stride,
+                         any ? (uint32_t)((rows - 1) * stride) + (uint32_t)(valid * kES) : 0);
     }
     return s;
   }
@@ -151,24 +157,23 @@ struct Operand {
     load_to_lds(s.rsrc, in ? offset[i] : kNoRead, s.at + (uint32_t)(i * WAVES * 1024));
   }
 
-  // The fragment of k part `part` (of STEP / 32) and the 32 rows from `first` on.
+  // The fragment of k part `part` (of STEP / 64) and the 16 rows from `first` on.
   __device__ static __forceinline__ Int4 fragment(const char *lds, int first, int part) {
-    const int l = (int)threadIdx.x & 63;
+    const int l = (int)threadIdx.x & 63, g = l >> 4;
     if constexpr (!ACROSS) {
-      return *reinterpret_cast<const Int4 *>(lds + (first + (l & 31)) * STEP +
-                                             (place_of(part * 2 + (l >> 5), l & 31) << 4));
+      return *reinterpret_cast<const Int4 *>(lds + (first + (l & 15)) * STEP +
+                                             (place_of(part * 4 + g, l & 15) << 4));
     } else if constexpr (kES == 2) {
-      const int k = part * 16 + (l >> 5) * 8 + ((l & 15) >> 2);
-      const int m = first + ((l >> 4) & 1) * 16 + (l & 3) * 4;
-      const int c = place_of(m >> 3, k);
-      const char *p = lds + k * kRowBytes + (c << 4) + (m & 4) * 2;
+      const int k = part * 32 + g * 8 + ((l & 15) >> 2), m = first + (l & 3) * 4;
+      const char *p = lds + k * kRowBytes + (place_of(m >> 3, k) << 4) + (m & 4) * 2;
       typedef __attribute__((address_space(3))) Short4 *LdsShort4;
       const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(p));
       const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsShort4)(p + 4 * kRowBytes));
       typedef short Short8 __attribute__((ext_vector_type(8)));
       return __builtin_bit_cast(Int4, (Short8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
-      const char *p = lds + (part * 8 + (l >> 5) * 4) * kRowBytes + (first + (l & 31)) * 4;
+      const int k = part * 16 + g * 4, m = first + (l & 15);
+      const char *p = lds + k * kRowBytes + (place_of(m >> 2, k) << 4) + (m & 3) * 4;
       Int4 f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const int *>(p + j * kRowBytes);
@@ -177,13 +182,15 @@ struct Operand {
   }
 };
 
+// In every wave: all reads of LDS have arrived, and all but the last VM loads
+// to it have landed.
 template <int VM>
 __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(VM) : "memory");
 }
 
 // A tile's shape: BM x BN per workgroup, WM x WN per wave; STEP bytes of k at
-// a time, STAGES (at least 3) of them in LDS.
+// a time, STAGES of them in LDS.
 template <typename T_, int BM_, int BN_, int WM_, int WN_, bool A_ACROSS, bool B_ACROSS, int STEP,
           int STAGES>
 struct Tile {
@@ -191,42 +198,35 @@ struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int kWavesM = BM / WM, kWavesN = BN / WN, kWaves = kWavesM * kWavesN;
   static constexpr int kThreads = kWaves * 64;
-  static constexpr int MI = WM / 32, NI = WN / 32;
+  static constexpr int MI = WM / 16, NI = WN / 16;
   using A = Operand<T, BM, A_ACROSS, kWaves, STEP>;
   using B = Operand<T, BN, B_ACROSS, kWaves, STEP>;
-  static constexpr int kStep = A::kStep, kParts = STEP / 32;
+  static constexpr int kStep = A::kStep, kParts = STEP / 64;
   static constexpr int kStage = A::kBytes + B::kBytes;
   static constexpr int kLds = STAGES * kStage;
-  static_assert(kLds <= 160 * 1024 && STAGES >= 3 && kParts % 2 == 0, "tile shape");
+  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && MI >= 2, "tile shape");
 
   // acc[mi][ni] += products of k in [k_begin, k_end); k_begin is a multiple of
   // kStep.  Every thread of the workgroup calls it; LDS is free at its end.
   //
-  // Step k is read while those up to k + STAGES - 1 load.  Fragments are read
-  // one part ahead of the products that use them, the first part of a step
-  // during the last products of the step before: there stands the step's one
-  // barrier, when every wave has read the last of its buffer and the next
-  // step's loads have landed.  Reads and loads are dealt out among the
-  // products (A's loads to the first part, B's to the last), so that no more
-  // than a few are issued between two of them: the matrix cores multiply on
-  // meanwhile.
+  // Fragments are read one part ahead of the products that use them: a row of
+  // blocks done, its A fragment of the next part is read in its place.  A step
+  // has one barrier, in its last part: every wave has read all of the step, into
+  // whose buffer the loads of step k + STAGES go from there on, and step k + 1
+  // has landed in every wave and is read from there on.  (It stands behind the
+  // part's first row of blocks, by which the last reads have arrived.)  Reads
+  // and loads are dealt out among the products, so that no more than a few are
+  // issued between two of them and the matrix cores multiply on.
   __device__ static __forceinline__ void walk(const A &a, const B &b, int64_t k_begin,
-                                              int64_t k_end, char *lds, Acc16 (&acc)[MI][NI]) {
+                                              int64_t k_end, char *lds, Acc4 (&acc)[MI][NI]) {
     const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / kWavesN * WM, wn = wave % kWavesN * WN;
     const uint32_t lds_at =
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    constexpr int kReads = MI + NI;
-    Int4 fa[2][MI], fb[2][NI];
-    auto read = [&](const char *cur, int part, int set, int i) {
-      if (i < NI)
-        fb[set][i] = B::fragment(cur + A::kBytes, wn + i * 32, part);
-      else
-        fa[set][i - NI] = A::fragment(cur, wm + (i - NI) * 32, part);
-    };
-    for (int s = 0; s < STAGES - 1; ++s) {
+    constexpr int kLoads = A::kLoads + B::kLoads;
+    Int4 fa[MI], fb[2][NI];
+    for (int s = 0; s < STAGES; ++s) {
       const int64_t k = k_begin + s * kStep;
-      if (k >= k_end) break;
       const auto sa = a.step(k, k_end, lds_at + (uint32_t)(s * kStage));
       const auto sb = b.step(k, k_end, lds_at + (uint32_t)(s * kStage + A::kBytes));
 #pragma unroll
@@ -234,52 +234,63 @@ struct Tile {
 #pragma unroll
       for (int i = 0; i < B::kLoads; ++i) b.load(sb, i);
     }
-    wait_and_meet<0>();
+    wait_and_meet<(STAGES - 1) * kLoads>();
 #pragma unroll
-    for (int i = 0; i < kReads; ++i) read(lds, 0, 0, i);
+    for (int j = 0; j < NI; ++j) fb[0][j] = B::fragment(lds + A::kBytes, wn + j * 16, 0);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa[i] = A::fragment(lds, wm + i * 16, 0);
     int buf = 0;
-    // MORE: there is a step to load.
-    auto one_step = [&](int64_t k, auto more) {
-      constexpr bool MORE = decltype(more)::value;
+    // SET: the half of fb that holds the step's first part.
+    auto one_step = [&](int64_t k, auto first_set) {
+      constexpr int SET = decltype(first_set)::value;
       const int next = buf + 1 == STAGES ? 0 : buf + 1;
       const char *cur = lds + buf * kStage, *then = lds + next * kStage;
-      typename A::Step sa;
-      typename B::Step sb;
-      if constexpr (MORE) {
-        const uint32_t at = lds_at + (uint32_t)((buf == 0 ? STAGES - 1 : buf - 1) * kStage);
-        sa = a.step(k + (STAGES - 1) * kStep, k_end, at);
-        sb = b.step(k + (STAGES - 1) * kStep, k_end, at + A::kBytes);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t at = lds_at + (uint32_t)(buf * kStage);
+      const auto sa = a.step(k + STAGES * kStep, k_end, at);
+      const auto sb = b.step(k + STAGES * kStep, k_end, at + A::kBytes);
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
-        const int set = part & 1;
-        if (part == kParts - 1)
-          wait_and_meet<MORE ? (STAGES - 3) * (A::kLoads + B::kLoads) + A::kLoads : 0>();
+        const bool last = part == kParts - 1;
+        const int set = (SET + part) & 1;
+        const char *from = last ? then : cur;
+        const int np = last ? 0 : part + 1;
+        // Rows of blocks beside which reads and loads are issued.
+        const int r0 = last ? 1 : 0, rows = MI - r0;
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          if constexpr (MORE) {
-            if (part == 0)
-#pragma unroll
-              for (int e = i * A::kLoads / MI; e < (i + 1) * A::kLoads / MI; ++e) a.load(sa, e);
-            if (part == kParts - 1)
-#pragma unroll
-              for (int e = i * B::kLoads / MI; e < (i + 1) * B::kLoads / MI; ++e) b.load(sb, e);
+          __builtin_amdgcn_sched_barrier(0);
+          if (last && i == 1) {
+            wait_and_meet<(STAGES - 2) * kLoads>();
+            fa[0] = A::fragment(from, wm, np);
           }
+          if (last && i >= r0)
 #pragma unroll
-          for (int e = i * kReads / MI; e < (i + 1) * kReads / MI; ++e)
-            read(part < kParts - 1 ? cur : then, part < kParts - 1 ? part + 1 : 0, set ^ 1, e);
+            for (int e = (i - r0) * kLoads / rows; e < (i - r0 + 1) * kLoads / rows; ++e)
+              if (e < A::kLoads) a.load(sa, e); else b.load(sb, e - A::kLoads);
+          if (i >= r0)
+#pragma unroll
+            for (int j = (i - r0) * NI / rows; j < (i - r0 + 1) * NI / rows; ++j)
+              fb[set ^ 1][j] = B::fragment(from + A::kBytes, wn + j * 16, np);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(fa[set][i], fb[set][j], acc[i][j]);
-          __builtin_amdgcn_sched_barrier(0);
+          for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(fa[i], fb[set][j], acc[i][j]);
+          if (i >= r0) fa[i] = A::fragment(from, wm + i * 16, np);
         }
       }
       buf = next;
     };
-    int64_t k = k_begin;
-    for (; k + (STAGES - 1) * kStep < k_end; k += kStep) one_step(k, std::true_type());
-    for (; k < k_end; k += kStep) one_step(k, std::false_type());
+    // Steps of one part go by two, so that fb's halves stay where they are;
+    // loads and products beyond k_end are of zeros.
+    if constexpr (kParts & 1) {
+      for (int64_t k = k_begin; k < k_end; k += 2 * kStep) {
+        one_step(k, std::integral_constant<int, 0>());
+        one_step(k + kStep, std::integral_constant<int, 1>());
+      }
+    } else {
+      for (int64_t k = k_begin; k < k_end; k += kStep)
+        one_step(k, std::integral_constant<int, 0>());
+    }
+    __builtin_amdgcn_sched_barrier(0);
     wait_and_meet<0>();
   }
 
@@ -295,17 +306,15 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
+      for (int j = 0; j < NI; ++j) {
+        const int n = wn + j * 16 + (l & 15), m = wm + i * 16 + (l >> 4) * 4;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 v;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = wn + j * 32 + (l & 31), m = wm + i * 32 + q * 8 + (l >> 5) * 4;
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = value(i, j, q * 4 + e);
-          const int at = m * (int)sizeof(T), c = (at >> 4) ^ (n & (kOutChunks - 1));
-          *reinterpret_cast<T4 *>(lds + n * kOutRow + (c << 4) + (at & 15)) = v;
-        }
+        for (int r = 0; r < 4; ++r) v[r] = value(i, j, r);
+        const int at = m * (int)sizeof(T), c = (at >> 4) ^ (n & (kOutChunks - 1));
+        *reinterpret_cast<T4 *>(lds + n * kOutRow + (c << 4) + (at & 15)) = v;
+      }
   }
   // Calls f(n, m, the 16 bytes of T at m ..) for the chunks of this thread.
   template <typename F>

@@ -211,7 +211,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
   a.init(weight, w_stride, v0, vocab);
   b.init(packed + pc.begin * wide, wide, r0,
          kPacked ? (pc.rows + kRowPad - 1) / kRowPad * kRowPad : pc.rows);
-  Acc16 acc[TL::MI][TL::NI] = {};
+  Acc4 acc[TL::MI][TL::NI] = {};
   TL::walk(a, b, 0, width, lds, acc);
 
   const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
@@ -225,8 +225,8 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
 #pragma unroll
       for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          acc[i][j][r] = f(acc[i][j][r], wm + i * 32 + (r >> 2) * 8 + (l >> 5) * 4 + (r & 3));
+        for (int r = 0; r < 4; ++r)
+          acc[i][j][r] = f(acc[i][j][r], wm + i * 16 + (l >> 4) * 4 + r);
   };
   if (softcap > 0.f) {
     const float to_exp = 2.f * kLog2E / softcap;
@@ -234,28 +234,29 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
   }
   if (v0 + TL::BM > vocab)
     each([&](float z, int v) { return v0 + v < vocab ? z : -INFINITY; });
-  // A lane holds rows wn + 32 j + l % 32 and every other group of four classes;
-  // lanes l and l + 32 and the waves along m share a row.
+  // A lane holds rows wn + 16 j + l % 16 and four classes of each 16; the lanes
+  // of equal l % 16 and the waves along m share a row.
   float *part = reinterpret_cast<float *>(lds);  // [kWavesM][BN]
   float top[TL::NI];
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
-    const int n = wn + j * 32 + (l & 31);
+    const int n = wn + j * 16 + (l & 15);
     const Label y = (r0 + n < pc.rows ? lab[pc.begin + r0 + n] : -1) - v0 - wm;
     if (__any(y >= 0 && y < TL::WM)) {
 #pragma unroll
       for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (i * 32 + (r >> 2) * 8 + (l >> 5) * 4 + (r & 3) == y) z_label[r0 + n] = acc[i][j][r];
+        for (int r = 0; r < 4; ++r)
+          if (i * 16 + (l >> 4) * 4 + r == y) z_label[r0 + n] = acc[i][j][r];
     }
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[i][j][r]);
+    m = fmaxf(m, __shfl_xor(m, 16));
     top[j] = fmaxf(m, __shfl_xor(m, 32));
-    if (TL::kWavesM > 1 && l < 32) part[wave / TL::kWavesN * TL::BN + n] = top[j];
+    if (TL::kWavesM > 1 && l < 16) part[wave / TL::kWavesN * TL::BN + n] = top[j];
   }
   if constexpr (TL::kWavesM > 1) {
     __syncthreads();
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
     for (int j = 0; j < TL::NI; ++j)
 #pragma unroll
       for (int w = 0; w < TL::kWavesM; ++w)
-        top[j] = fmaxf(top[j], part[w * TL::BN + wn + j * 32 + (l & 31)]);
+        top[j] = fmaxf(top[j], part[w * TL::BN + wn + j * 16 + (l & 15)]);
     __syncthreads();
   }
 #pragma unroll
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
+      for (int r = 0; r < 4; ++r) {
         const float z = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(z, kLog2E, base));
         s += e;
         if (!P) continue;
@@ -284,14 +285,15 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
           acc[i][j][r] = e * kExpScale<T>;
         }
       }
+    s += __shfl_xor(s, 16);
     s += __shfl_xor(s, 32);
-    if (l < 32) part[wave / TL::kWavesN * TL::BN + wn + j * 32 + l] = s;
+    if (l < 16) part[wave / TL::kWavesN * TL::BN + wn + j * 16 + l] = s;
   }
   __syncthreads();
-  if (wm == 0 && l < 32)
+  if (wm == 0 && l < 16)
 #pragma unroll
     for (int j = 0; j < TL::NI; ++j) {
-      const int n = wn + j * 32 + l;
+      const int n = wn + j * 16 + l;
       float s = part[n];
       for (int w = 1; w < TL::kWavesM; ++w) s += part[w * TL::BN + n];
       if (r0 + n < pc.rows) stats[(int64_t)(r0 + n) * tiles + at.slow] = make_float2(top[j], s);
@@ -483,26 +485,21 @@ __global__ __launch_bounds__(TL::kThreads) void k_d_hidden(
   typename TL::B b;
   a.init(weight, w_stride, d0, width);
   b.init(P, ldp, r0, (pc.rows + kRowPad - 1) / kRowPad * kRowPad);
-  Acc16 acc[TL::MI][TL::NI] = {};
+  Acc4 acc[TL::MI][TL::NI] = {};
   TL::walk(a, b, (int64_t)split * split_v, min((int64_t)(split + 1) * split_v, (int64_t)vocab), lds,
            acc);
   const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
   const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
-    const int32_t r = r0 + wn + j * 32 + (l & 31);
+    const int32_t r = r0 + wn + j * 16 + (l & 15);
     if (r >= pc.rows) continue;
     float *out = part + (int64_t)split * part_stride + (int64_t)r * wide;
 #pragma unroll
-    for (int i = 0; i < TL::MI; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int32_t d = d0 + wm + i * 32 + q * 8 + (l >> 5) * 4;
-        if (d < wide)
-          *reinterpret_cast<float4 *>(out + d) =
-              make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                          acc[i][j][4 * q + 3]);
-      }
+    for (int i = 0; i < TL::MI; ++i) {
+      const int32_t d = d0 + wm + i * 16 + (l >> 4) * 4;
+      if (d < wide) *reinterpret_cast<Acc4 *>(out + d) = acc[i][j];
+    }
   }
 }
 
@@ -557,34 +554,23 @@ __global__ __launch_bounds__(TL::kThreads) void k_d_weight(
   typename TL::B b;
   a.init(packed + (int64_t)pc.begin * wide, wide, d0, wide);
   b.init(P, ldp, v0, (int32_t)ldp);
-  Acc16 acc[TL::MI][TL::NI] = {};
+  Acc4 acc[TL::MI][TL::NI] = {};
   TL::walk(a, b, 0, (pc.rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
   if (pieces > 1) {
     const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
     const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
 #pragma unroll
     for (int j = 0; j < TL::NI; ++j) {
-      const int32_t v = v0 + wn + j * 32 + (l & 31);
+      const int32_t v = v0 + wn + j * 16 + (l & 15);
       if (v >= vocab) continue;
 #pragma unroll
-      for (int i = 0; i < TL::MI; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int32_t d = d0 + wm + i * 32 + q * 8 + (l >> 5) * 4;
-          if (d >= wide) continue;
-          float4 *p = reinterpret_cast<float4 *>(sum + (int64_t)v * wide + d);
-          float4 x = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                                 acc[i][j][4 * q + 3]);
-          if (piece > 0) {
-            const float4 y = *p;
-            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-            acc[i][j][4 * q] = x.x;
-            acc[i][j][4 * q + 1] = x.y;
-            acc[i][j][4 * q + 2] = x.z;
-            acc[i][j][4 * q + 3] = x.w;
-          }
-          if (piece < pieces - 1) *p = x;
-        }
+      for (int i = 0; i < TL::MI; ++i) {
+        const int32_t d = d0 + wm + i * 16 + (l >> 4) * 4;
+        if (d >= wide) continue;
+        Acc4 *p = reinterpret_cast<Acc4 *>(sum + (int64_t)v * wide + d);
+        if (piece > 0) acc[i][j] += *p;
+        if (piece < pieces - 1) *p = acc[i][j];
+      }
     }
     if (piece < pieces - 1) return;
   }
@@ -642,8 +628,8 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const HeadInfo *info, const i
 enum Shape : int32_t { kBig, kMid, kThin };
 template <typename T, Shape S, bool A_ACROSS, bool B_ACROSS>
 using TileOf = std::conditional_t<
-    S == kBig, Tile<T, 256, 256, 128, 64, A_ACROSS, B_ACROSS, 64, 4>,
-    std::conditional_t<S == kMid, Tile<T, 128, 128, 64, 64, A_ACROSS, B_ACROSS, 64, 4>,
+    S == kBig, Tile<T, 256, 256, 128, 64, A_ACROSS, B_ACROSS, 128, 2>,
+    std::conditional_t<S == kMid, Tile<T, 128, 128, 64, 64, A_ACROSS, B_ACROSS, 128, 2>,
                        Tile<T, 128, 32, 32, 32, A_ACROSS, B_ACROSS, 128, 3>>>;
 constexpr int shape_m(Shape s) { return s == kBig ? 256 : 128; }
 constexpr int shape_n(Shape s) { return s == kBig ? 256 : s == kMid ? 128 : 32; }
@@ -711,7 +697,9 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
     // d_hidden's sums run over the whole vocabulary, in parts that fill the
     // CUs.  What a number of parts costs, in microseconds: rounds of tiles (a
     // CU holds one kBig, two kMid or kThin), each with a start and an end, and
-    // the parts' sums written and read.  The rates are the kernels' own.
+    // the parts' sums written and read.  The rates are the kernels' own.  How
+    // many rows count is not known here: the mean over half, three quarters and
+    // all of them.
     const int64_t step = 128 / es, steps = (vocab + step - 1) / step;
     const int64_t tiles = tiles_of(p.d_hidden, width, piece);
     const int64_t at_once = p.d_hidden == kBig ? kCus : 2 * kCus;
@@ -719,9 +707,11 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
     const double part_us = (double)piece * p.wide * 8 / 4e6;
     double best = 0.0;
     for (int64_t n = 1; n <= std::min<int64_t>(64, std::max<int64_t>(1, steps / 4)); ++n) {
-      const double us = (double)((tiles * n + at_once - 1) / at_once) *
-                            ((double)((steps + n - 1) / n) * step_us + 6.0) +
-                        (double)n * part_us;
+      double rounds = 0.0;
+      for (int64_t share = 2; share <= 4; ++share)
+        rounds += (double)((tiles * share / 4 * n + at_once - 1) / at_once) * 4 / share / 3;
+      const double us =
+          rounds * ((double)((steps + n - 1) / n) * step_us + 6.0) + (double)n * part_us;
       if (n == 1 || us < best) {
         best = us;
         p.splits = (int32_t)n;
@@ -729,7 +719,7 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
     }
     p.split_v = (int32_t)((steps + p.splits - 1) / p.splits * step);
     p.splits = (int32_t)((vocab + p.split_v - 1) / p.split_v);
-    p.d_weight = !f32 && tiles_of(kBig, width, vocab) >= kCus ? kBig : kMid;
+    p.d_weight = shape(width, vocab);
   }
   // Loads are of 16 bytes, within 2^31 bytes of a tile's first row.
   p.pack_weight = ((uintptr_t)weight & 15) || w_stride * es % 16 || width * es % 16 ||
@@ -772,12 +762,11 @@ struct HeadCall {
 
 // f(std::integral_constant<Shape, s>) for s; float32 has no 256 x 256 tile
 // (its output would not fit LDS).
-template <typename T, bool THIN, typename F>
+template <typename T, typename F>
 void by_shape(Shape s, F &&f) {
   if constexpr (sizeof(T) == 2)
     if (s == kBig) return f(std::integral_constant<Shape, kBig>());
-  if constexpr (THIN)
-    if (s == kThin) return f(std::integral_constant<Shape, kThin>());
+  if (s == kThin) return f(std::integral_constant<Shape, kThin>());
   f(std::integral_constant<Shape, kMid>());
 }
 
@@ -838,7 +827,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
   const int dh_vec =
       (uintptr_t)c.d_hidden % (4 * sizeof(T)) == 0 && c.dh_stride % 4 == 0;
   for (int32_t k = 0; k < p.pieces; ++k) {
-    by_shape<T, true>(p.scores, [&](auto s) {
+    by_shape<T>(p.scores, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, false, false>;
       k_scores<TL, int32_t><<<(unsigned)tiles_of(s, p.vocab, piece), TL::kThreads, 0, st>>>(
           weight, w_stride, p.vocab, w_width, packed, p.wide, lab, info, k, p.pieces, c.softcap,
@@ -848,7 +837,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
         info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
         z_label, P, p.ldp, c.row_loss, c.lse);
     if (!c.grad) continue;
-    by_shape<T, true>(p.d_hidden, [&](auto s) {
+    by_shape<T>(p.d_hidden, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, true, false>;
       k_d_hidden<TL><<<(unsigned)(tiles_of(s, w_width, piece) * p.splits), TL::kThreads, 0, st>>>(P, p.ldp, weight, w_stride, p.vocab, w_width,
                                                 p.wide, info, k, p.pieces, p.splits, p.split_v,
@@ -857,7 +846,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
     k_d_hidden_sum<T><<<(unsigned)piece, 256, 0, st>>>(
         info, k, p.pieces, idx, p.splits, part, part_stride, p.wide, p.width,
         static_cast<T *>(c.d_hidden), c.dh_stride, dh_vec);
-    by_shape<T, false>(p.d_weight, [&](auto s) {
+    by_shape<T>(p.d_weight, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, true, true>;
       k_d_weight<TL><<<(unsigned)tiles_of(s, p.width, 1) *
                            (unsigned)((p.vocab + TL::BN - 1) / TL::BN),
