@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from collections import namedtuple
 
 from . import _native
@@ -150,8 +151,6 @@ def linear_softmax_grad(hidden, weight, labels, *, row_weight=None, reduction="m
 
 def _dense(t):
     """Whether t's values fill one block of memory, in whatever order."""
-    if t.is_contiguous():
-        return True
     size = 1
     for stride, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
         if stride != size:
@@ -161,54 +160,68 @@ def _dense(t):
 
 
 def _list(torch, tensors, what):
-    tensors = list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{what} must be torch tensors, got {type(t).__name__}")
+    """(addresses, lengths, dtype codes, GPU) of the tensors as arrays for the
+    C ABI.  Lists are long and the kernels short: one pass of the tensors'
+    methods each, and no loop of Python statements unless something is odd."""
     if not tensors:
         raise ValueError(f"{what} is empty")
-    codes = [_dtype_codes.get(t.dtype, -1) for t in tensors]
-    if min(codes) < 0:
+    Tensor = torch.Tensor
+    try:
+        ptrs = array("Q", map(Tensor.data_ptr, tensors))
+        lengths = array("q", map(Tensor.numel, tensors))
+        devices = set(map(Tensor.get_device, tensors))
+        dense = all(map(Tensor.is_contiguous, tensors))
+        dtypes = [t.dtype for t in tensors]
+    except (TypeError, RuntimeError):
+        bad = [t for t in tensors if not isinstance(t, Tensor)]
+        if not bad:
+            raise
+        raise ValueError(f"{what} must be torch tensors, got {type(bad[0]).__name__}") from None
+    kinds = set(dtypes)
+    if not kinds <= _dtype_codes.keys():
         raise ValueError(f"{what} must be bfloat16, float16 or float32, got "
-                         f"{tensors[codes.index(-1)].dtype}")
-    dev = tensors[0].get_device()
-    if dev < 0 or any(t.get_device() != dev for t in tensors):
+                         f"{(kinds - _dtype_codes.keys()).pop()}")
+    if len(devices) != 1 or min(devices) < 0:
         raise ValueError(f"{what} must all be on one GPU")
-    for t in tensors:
-        if not _dense(t):
-            raise ValueError(f"{what} must be dense: a tensor of shape {tuple(t.shape)} has "
-                             f"strides {t.stride()}")
-    return tensors, codes, dev
+    if not dense:
+        for t in tensors:
+            if not t.is_contiguous() and not _dense(t):
+                raise ValueError(f"{what} must be dense: a tensor of shape {tuple(t.shape)} has "
+                                 f"strides {t.stride()}")
+    if len(kinds) == 1:
+        codes = array("i", [_dtype_codes[dtypes[0]]]) * len(tensors)
+    else:
+        codes = array("i", map(_dtype_codes.__getitem__, dtypes))
+    return ptrs, lengths, codes, devices.pop()
 
 
 def _norm(tensors, inv_scale, max_norm, out):
     torch = _torch()
-    tensors, codes, dev = _list(torch, tensors, "tensors")
+    tensors = list(tensors)
+    ptrs, lengths, codes, index = _list(torch, tensors, "tensors")
     n = len(tensors)
-    ptrs = [t.data_ptr() for t in tensors]
-    outs = None
-    if max_norm is not None:
-        outs = ptrs
-        if out is not None:
-            out, out_codes, out_dev = _list(torch, out, "out")
-            if len(out) != n or out_codes != codes or out_dev != dev or any(
-                    o.shape != t.shape or o.stride() != t.stride() for o, t in zip(out, tensors)):
-                raise ValueError("out must match tensors in number, shape, strides, dtype and GPU")
-            outs = [t.data_ptr() for t in out]
-    lengths = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
-    codes = (ctypes.c_int32 * n)(*codes)
-    ptrs = (ctypes.c_void_p * n)(*ptrs)
-    dev = torch.device("cuda", dev)
+    outs = ptrs
+    if out is not None:
+        out = list(out)
+        outs, _, out_codes, out_index = _list(torch, out, "out")
+        if len(out) != n or out_codes != codes or out_index != index or any(
+                o.shape != t.shape or o.stride() != t.stride() for o, t in zip(out, tensors)):
+            raise ValueError("out must match tensors in number, shape, strides, dtype and GPU")
+
+    def at(a):
+        return a.buffer_info()[0]
+
+    dev = torch.device("cuda", index)
     L = _native.lib()
-    ws = _workspace(torch, dev, L.bsscl_grad_norm_workspace, n, lengths)
+    ws = _workspace(torch, dev, L.bsscl_grad_norm_workspace, n, at(lengths))
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    args = (dev.index, _stream(torch, dev), n, ptrs)
-    if outs is None:
-        _native.check(L.bsscl_grad_norm(*args, lengths, codes, float(inv_scale), norm.data_ptr(),
-                                        ws.data_ptr(), ws.numel()))
+    args = (index, _stream(torch, dev), n, at(ptrs))
+    if max_norm is None:
+        _native.check(L.bsscl_grad_norm(*args, at(lengths), at(codes), float(inv_scale),
+                                        norm.data_ptr(), ws.data_ptr(), ws.numel()))
     else:
-        _native.check(L.bsscl_clip_grads(*args, (ctypes.c_void_p * n)(*outs), lengths, codes,
-                                         float(inv_scale), float(max_norm), norm.data_ptr(),
+        _native.check(L.bsscl_clip_grads(*args, at(outs), at(lengths), at(codes),
+                                         float(inv_scale), max_norm, norm.data_ptr(),
                                          ws.data_ptr(), ws.numel()))
     return norm
 
