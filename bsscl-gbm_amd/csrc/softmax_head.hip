@@ -33,7 +33,7 @@ constexpr int64_t kPieceBytes = int64_t(1) << 30;
 
 struct HeadInfo {
   int32_t rows;      // counting rows
-  float to_operand;  // power of two on d loss / d score in the operands (float16)
+  float to_operand;  // what d loss / d score is multiplied by as an operand
   float from_operand;
 };
 
@@ -90,7 +90,7 @@ struct PrepareArgs {
   const float *row_weight;
   int32_t rows, vocab, mean;
   float grad_scale;
-  int32_t narrow;
+  int32_t whole, narrow;  // float32, float16
   int32_t *idx, *lab;
   float *u;
   int32_t *pos;
@@ -141,16 +141,18 @@ __device__ void prepare(const PrepareArgs &a, double *tmp) {
   big = block_fold<THREADS>(big, tmp, [](double x, double y) { return fmax(x, y); });
   const double share = a.mean ? (sum != 0.0 ? 1.0 / sum : 0.0) : 1.0;
   if (tid == 0) {
-    // The largest weight at 2^10 to 2^11 leaves a factor of 2^5 to float16's
-    // largest value (1 + 2 zeta lse may exceed 1) and its smallest at 2^-35 of
-    // the weight.
-    int e = 0;
-    const float m = (float)(big * fabs(share)) * fabsf(a.grad_scale);
-    if (a.narrow && m > 0.f && m < INFINITY) e = 10 - ilogbf(m);
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    // The largest weight becomes 1: rows of that weight (all rows, where none
+    // are given) then have d loss / d label score at p - 1, which bf16 and
+    // float16 hold to p for surprising labels, and not off by half a step like
+    // any other multiple.  In float16 it becomes 2^10: a factor of 2^5 and more
+    // is left to the largest value (1 + 2 zeta lse may exceed 1), and the
+    // smallest lies at 2^-35 of the weight.
+    float m = (float)(big * fabs(share)) * fabsf(a.grad_scale);
+    if (!(m >= 0x1p-100f && m <= 0x1p100f)) m = 1.f;
+    const float one = a.narrow ? 1024.f : 1.f;
     a.info->rows = base;
-    a.info->to_operand = ldexpf(1.f, e);
-    a.info->from_operand = ldexpf(1.f, -e);
+    a.info->to_operand = a.whole ? 1.f : one / m;
+    a.info->from_operand = a.whole ? 1.f : m / one;
   }
   if (a.mean)
     for (int32_t p = tid; p < base; p += THREADS) a.u[p] = (float)((double)a.u[p] * share);
@@ -262,6 +264,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
         for (int r = 0; r < 4; ++r)
           acc[i][j][r] = f(acc[i][j][r], wm + i * 16 + (l >> 4) * 4 + r);
   };
+  const float to_slope = softcap > 0.f ? 1.f / softcap : 0.f;
   if (softcap > 0.f) {
     const float to_exp = 2.f * kLog2E / softcap;
     each([&](float z, int) { return softcap * tanh_of(z, to_exp); });
@@ -313,7 +316,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
         s += e;
         if (!P) continue;
         if (softcap > 0.f) {
-          const float t = e > 0.f ? z / softcap : 0.f;
+          const float t = e > 0.f ? z * to_slope : 0.f;
           acc[i][j][r] = e * (kExpScale<T> - kExpScale<T> * t * t);
         } else {
           acc[i][j][r] = e * kExpScale<T>;
@@ -443,8 +446,8 @@ template <typename T>
 __global__ __launch_bounds__(kRowThreads) void k_rows(
     const HeadInfo *info, int32_t piece, int32_t pieces, const int32_t *idx, const int32_t *lab,
     const float *u, float softcap, float z_loss, float grad_scale, int32_t tiles, int32_t tile_v,
-    const float2 *stats, const float *z_label, T *P, int64_t ldp, float *row_loss,
-    float *lse_out) {
+    const float2 *stats, const float *z_label, T *P, int64_t ldp, float *own_rest,
+    float *row_loss, float *lse_out) {
   __shared__ float red[2 * kRowThreads / 64];
   constexpr int kVec = 16 / (int)sizeof(T), kVecs = 4;
   const Piece pc = piece_of(info->rows, piece, pieces);
@@ -471,6 +474,9 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
   const float py = expm1f(zy - lse);
   const float slope = softcap > 0.f ? 1.f - (zy / softcap) * (zy / softcap) : 1.f;
   const float own = g * slope * (py + zl * (py + 1.f));
+  // What rounding takes of the label's value, the row's largest as a rule:
+  // k_d_hidden_sum adds it times the label's row of the weight.
+  if (tid == 0) own_rest[r] = own - (float)from_float<T>(own);
   const float scale = g * (1.f + zl) / kExpScale<T>;
   const int tile_shift = 31 - __clz(tile_v / kVec);
   for (int32_t i0 = tid; i0 < n; i0 += kRowThreads * kVecs) {
@@ -558,14 +564,14 @@ __global__ __launch_bounds__(1024) void k_loss_sum(const LossArgs a) {
   loss_sum<1024>(a, tmp);
 }
 
-// The parts of d_hidden added up in their order, into the rows' places; block 0
-// adds up the loss (of the last piece, when all rows have theirs).
+// The parts of d_hidden added up in their order, into the rows' places, with
+// what rounding took of the label's value; block 0 adds up the loss (of the last
+// piece, when all rows have theirs).
 template <typename T>
-__global__ __launch_bounds__(256) void k_d_hidden_sum(int32_t piece, int32_t pieces,
-                                                      const LossArgs loss, int32_t splits,
-                                                      const float *part, int64_t part_stride,
-                                                      int32_t wide, int32_t width, T *d_hidden,
-                                                      int64_t d_stride, int32_t vec) {
+__global__ __launch_bounds__(256) void k_d_hidden_sum(
+    int32_t piece, int32_t pieces, const LossArgs loss, int32_t splits, const float *part,
+    int64_t part_stride, int32_t wide, int32_t width, const int32_t *lab, const float *own_rest,
+    const T *weight, int64_t w_stride, T *d_hidden, int64_t d_stride, int32_t vec) {
   __shared__ double tmp[256];
   if (blockIdx.x == 0) {
     if (piece == pieces - 1) loss_sum<256>(loss, tmp);
@@ -577,15 +583,22 @@ __global__ __launch_bounds__(256) void k_d_hidden_sum(int32_t piece, int32_t pie
   if (r >= pc.rows) return;
   const float back = info->from_operand;
   T *row = d_hidden + (int64_t)loss.idx[pc.begin + r] * d_stride;
+  const T *own_row = weight + (int64_t)lab[pc.begin + r] * w_stride;
+  const float rest = own_rest[r];
+  typedef T T4 __attribute__((ext_vector_type(4)));
   for (int32_t d = (int32_t)threadIdx.x * 4; d < width; d += 1024) {
     const float *p = part + (int64_t)r * wide + d;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (rest != 0.f) {
+      const T4 w = *reinterpret_cast<const T4 *>(own_row + d);
+      s = make_float4(rest * (float)w[0], rest * (float)w[1], rest * (float)w[2],
+                      rest * (float)w[3]);
+    }
 #pragma unroll 4
     for (int32_t k = 0; k < splits; ++k) {
       const float4 x = *reinterpret_cast<const float4 *>(p + (int64_t)k * part_stride);
       s = make_float4(s.x + x.x, s.y + x.y, s.z + x.z, s.w + x.w);
     }
-    typedef T T4 __attribute__((ext_vector_type(4)));
     const T4 v = {(T)(s.x * back), (T)(s.y * back), (T)(s.z * back), (T)(s.w * back)};
     if (vec && d + 4 <= width) {
       *reinterpret_cast<T4 *>(row + d) = v;
@@ -696,7 +709,7 @@ struct HeadPlan {
   Shape scores, d_hidden, d_weight;
   bool pack_weight;
   int64_t ldp;
-  size_t info, idx, lab, u, pos, packed, stats, z_label, P, part, sum, weight, bytes;
+  size_t info, idx, lab, u, pos, packed, stats, z_label, own_rest, P, part, sum, weight, bytes;
 };
 
 // Grids stay below 2^32 threads, and what a tile loads within 2^31 bytes.
@@ -791,6 +804,7 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
   p.packed = take(round_up(rows, kRowPad) * p.wide * es);
   p.stats = take((int64_t)p.piece_rows * p.tiles * (int64_t)sizeof(float2));
   p.z_label = take((int64_t)p.piece_rows * 4);
+  p.own_rest = take(grad ? (int64_t)p.piece_rows * 4 : 0);
   p.P = take(grad ? (int64_t)p.piece_rows * p.ldp * es : 0);
   p.part = take(grad ? (int64_t)p.splits * p.piece_rows * p.wide * 4 : 0);
   p.sum = take(grad && p.pieces > 1 ? vocab * p.wide * 4 : 0);
@@ -839,6 +853,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
   auto *packed = reinterpret_cast<T *>(c.ws + p.packed);
   auto *stats = reinterpret_cast<float2 *>(c.ws + p.stats);
   auto *z_label = reinterpret_cast<float *>(c.ws + p.z_label);
+  auto *own_rest = reinterpret_cast<float *>(c.ws + p.own_rest);
   auto *P = c.grad ? reinterpret_cast<T *>(c.ws + p.P) : nullptr;
   auto *part = reinterpret_cast<float *>(c.ws + p.part);
   auto *sum = reinterpret_cast<float *>(c.ws + p.sum);
@@ -868,7 +883,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
     w_stride = w_width = p.wide;
   }
   const PrepareArgs prep{c.labels, c.row_weight, p.rows, p.vocab, c.mean, c.grad_scale,
-                         std::is_same<T, _Float16>::value, idx, lab, u, pos, c.row_loss, c.lse,
+                         sizeof(T) == 4, std::is_same<T, _Float16>::value, idx, lab, u, pos, c.row_loss, c.lse,
                          info};
   const bool count = p.rows <= kCountRows;
   if (!count) k_head_prepare<<<1, 1024, 0, st>>>(prep);
@@ -891,7 +906,7 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
     });
     k_rows<T><<<(unsigned)(c.grad ? p.piece_rows : piece), kRowThreads, 0, st>>>(
         info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
-        z_label, P, p.ldp, c.row_loss, c.lse);
+        z_label, P, p.ldp, own_rest, c.row_loss, c.lse);
     if (!c.grad) continue;
     by_shape<T>(p.d_hidden, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, true, false>;
@@ -900,8 +915,8 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
                                                 part, part_stride);
     });
     k_d_hidden_sum<T><<<(unsigned)piece + 1, 256, 0, st>>>(
-        k, p.pieces, loss, p.splits, part, part_stride, p.wide, p.width,
-        static_cast<T *>(c.d_hidden), c.dh_stride, dh_vec);
+        k, p.pieces, loss, p.splits, part, part_stride, p.wide, p.width, lab, own_rest, weight,
+        w_stride, static_cast<T *>(c.d_hidden), c.dh_stride, dh_vec);
     by_shape<T>(p.d_weight, [&](auto s) {
       using TL = TileOf<T, decltype(s)::value, true, true>;
       k_d_weight<TL><<<(unsigned)tiles_of(s, p.width, 1) *

@@ -507,10 +507,11 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
  *   d_hidden = d loss / d hidden (rows x width, stride d_hidden_stride) and
  *   d_weight = d loss / d weight (vocab x width, stride d_weight_stride),
  * both of the inputs' dtype and overwritten.
- * Sums run in float32; d loss / d score is rounded to the inputs' dtype once
- * it has been normalised, as operand of the two products.  In float16 it is
- * scaled by a power of two first (it holds at least 2^-35 of the largest row
- * weight), and 1 + 2 zeta lse may reach 32.
+ * Sums run in float32.  d loss / d score is rounded to the inputs' dtype as
+ * operand of the two products, divided by the largest row weight first (so that
+ * equal weights are exact); what that takes of the label's value is added to
+ * d_hidden again.  In float16 it holds at least 2^-35 of the largest row
+ * weight, and 1 + 2 zeta lse may reach 32.
  * 1 <= rows <= 8000000, 1 <= width <= 65536, 1 <= vocab <= 4000000.
  */
 int bsscl_head_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t vocab,
