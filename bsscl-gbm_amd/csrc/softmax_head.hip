@@ -505,42 +505,136 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
   }
 }
 
-// d_hidden of a piece: BM columns x BN rows over the `split`th part of the
-// vocabulary, as float32 sums of their own.
+// What the two products of a piece take.
+struct ProductArgs {
+  const void *P;
+  int64_t ldp;
+  const void *packed;
+  int32_t wide, vocab, width;
+  const HeadInfo *info;
+  int32_t piece, pieces;
+  // d_hidden: the weight (w_width columns), its vocabulary in `splits` parts
+  const void *weight;
+  int64_t w_stride;
+  int32_t w_width, splits, split_v;
+  float *part;
+  int64_t part_stride;
+  // d_weight
+  float *sum;
+  void *d_weight;
+  int64_t dw_stride;
+  int32_t dw_vec;
+};
+
+// d_hidden of a piece: BM columns x BN rows over a part of the vocabulary, as
+// float32 sums of their own.  Tile `block` of those there are.
 template <typename TL>
-__global__ __launch_bounds__(TL::kThreads) void k_d_hidden(
-    const typename TL::T *P, int64_t ldp, const typename TL::T *weight, int64_t w_stride,
-    int32_t vocab, int32_t width, int32_t wide, const HeadInfo *info, int32_t piece,
-    int32_t pieces, int32_t splits, int32_t split_v, float *part, int64_t part_stride) {
-  __shared__ __align__(1024) char lds[TL::kLds];
-  const Piece pc = piece_of(info->rows, piece, pieces);
+__device__ __forceinline__ void d_hidden_tile(const ProductArgs &g, uint32_t block, char *lds) {
+  using T = typename TL::T;
+  const T *P = static_cast<const T *>(g.P), *weight = static_cast<const T *>(g.weight);
+  const Piece pc = piece_of(g.info->rows, g.piece, g.pieces);
   const uint32_t row_tiles = (uint32_t)(pc.rows + TL::BN - 1) / TL::BN;
-  const uint32_t col_tiles = (uint32_t)(width + TL::BM - 1) / TL::BM;
-  const uint32_t each = row_tiles * col_tiles, total = each * (uint32_t)splits;
-  if (blockIdx.x >= total) return;
-  const uint32_t idx = xcd_order(blockIdx.x, total);
+  const uint32_t col_tiles = (uint32_t)(g.w_width + TL::BM - 1) / TL::BM;
+  const uint32_t each = row_tiles * col_tiles, total = each * (uint32_t)g.splits;
+  if (block >= total) return;
+  const uint32_t idx = xcd_order(block, total);
   const TileAt at = tile_at(idx % each, col_tiles, row_tiles);
   const int32_t d0 = at.slow * TL::BM, r0 = at.fast * TL::BN, split = (int32_t)(idx / each);
   typename TL::A a;
   typename TL::B b;
-  a.init(weight, w_stride, d0, width);
-  b.init(P, ldp, r0, (pc.rows + kRowPad - 1) / kRowPad * kRowPad);
+  a.init(weight, g.w_stride, d0, g.w_width);
+  b.init(P, g.ldp, r0, (pc.rows + kRowPad - 1) / kRowPad * kRowPad);
   Acc4 acc[TL::MI][TL::NI] = {};
-  TL::walk(a, b, (int64_t)split * split_v, min((int64_t)(split + 1) * split_v, (int64_t)vocab), lds,
-           acc);
+  TL::walk(a, b, (int64_t)split * g.split_v,
+           min((int64_t)(split + 1) * g.split_v, (int64_t)g.vocab), lds, acc);
   const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
   const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
     const int32_t r = r0 + wn + j * 16 + (l & 15);
     if (r >= pc.rows) continue;
-    float *out = part + (int64_t)split * part_stride + (int64_t)r * wide;
+    float *out = g.part + (int64_t)split * g.part_stride + (int64_t)r * g.wide;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i) {
       const int32_t d = d0 + wm + i * 16 + (l >> 4) * 4;
-      if (d < wide) *reinterpret_cast<Acc4 *>(out + d) = acc[i][j];
+      if (d < g.wide) *reinterpret_cast<Acc4 *>(out + d) = acc[i][j];
     }
   }
+}
+
+// d_weight of a piece: BM columns x BN classes over the piece's rows; pieces
+// before the last add up in float32.  Tile `block` of `blocks`.
+template <typename TL>
+__device__ __forceinline__ void d_weight_tile(const ProductArgs &g, uint32_t block,
+                                              uint32_t blocks, char *lds) {
+  using T = typename TL::T;
+  T *d_weight = static_cast<T *>(g.d_weight);
+  const int32_t wide = g.wide, vocab = g.vocab, width = g.width, piece = g.piece,
+                pieces = g.pieces;
+  const Piece pc = piece_of(g.info->rows, piece, pieces);
+  const uint32_t col_tiles = (uint32_t)(width + TL::BM - 1) / TL::BM;
+  const uint32_t v_tiles = (uint32_t)(vocab + TL::BN - 1) / TL::BN;
+  const TileAt at = tile_at(xcd_order(block, blocks), v_tiles, col_tiles);
+  const int32_t v0 = at.slow * TL::BN, d0 = at.fast * TL::BM;
+  typename TL::A a;
+  typename TL::B b;
+  a.init(static_cast<const T *>(g.packed) + (int64_t)pc.begin * wide, wide, d0, wide);
+  b.init(static_cast<const T *>(g.P), g.ldp, v0, (int32_t)g.ldp);
+  Acc4 acc[TL::MI][TL::NI] = {};
+  TL::walk(a, b, 0, (pc.rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
+  if (pieces > 1) {
+    const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
+    const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
+#pragma unroll
+    for (int j = 0; j < TL::NI; ++j) {
+      const int32_t v = v0 + wn + j * 16 + (l & 15);
+      if (v >= vocab) continue;
+#pragma unroll
+      for (int i = 0; i < TL::MI; ++i) {
+        const int32_t d = d0 + wm + i * 16 + (l >> 4) * 4;
+        if (d >= wide) continue;
+        Acc4 *p = reinterpret_cast<Acc4 *>(g.sum + (int64_t)v * wide + d);
+        if (piece > 0) acc[i][j] += *p;
+        if (piece < pieces - 1) *p = acc[i][j];
+      }
+    }
+    if (piece < pieces - 1) return;
+  }
+  const float back = g.info->from_operand;
+  TL::stage_out(lds, [&](int i, int j, int r) { return (T)(acc[i][j][r] * back); });
+  __syncthreads();
+  if (g.dw_vec) {
+    TL::read_out(lds, [&](int n, int m, Int4 x) {
+      if (v0 + n < vocab && d0 + m < width)
+        *reinterpret_cast<Int4 *>(d_weight + (int64_t)(v0 + n) * g.dw_stride + d0 + m) = x;
+    });
+  } else {
+    TL::read_out_one(lds, [&](int n, int m, T x) {
+      if (v0 + n < vocab && d0 + m < width) d_weight[(int64_t)(v0 + n) * g.dw_stride + d0 + m] = x;
+    });
+  }
+}
+
+template <typename TL>
+__global__ __launch_bounds__(TL::kThreads) void k_d_hidden(const ProductArgs g) {
+  __shared__ __align__(1024) char lds[TL::kLds];
+  d_hidden_tile<TL>(g, blockIdx.x, lds);
+}
+template <typename TL>
+__global__ __launch_bounds__(TL::kThreads) void k_d_weight(const ProductArgs g) {
+  __shared__ __align__(1024) char lds[TL::kLdsOut];
+  d_weight_tile<TL>(g, blockIdx.x, gridDim.x, lds);
+}
+// Both in one launch, d_hidden's long tiles (`hidden` blocks, a multiple of 8)
+// first: d_weight's short ones fill the CUs that they leave.
+template <typename TH, typename TW>
+__global__ __launch_bounds__(TH::kThreads) void k_products(const ProductArgs g, uint32_t hidden) {
+  static_assert(TH::kThreads == TW::kThreads);
+  __shared__ __align__(1024) char lds[TH::kLds > TW::kLdsOut ? TH::kLds : TW::kLdsOut];
+  if (blockIdx.x < hidden)
+    d_hidden_tile<TH>(g, blockIdx.x, lds);
+  else
+    d_weight_tile<TW>(g, blockIdx.x - hidden, gridDim.x - hidden, lds);
 }
 
 // loss = sum of u * row_loss over the counting rows, in their order.
@@ -607,59 +701,6 @@ __global__ __launch_bounds__(256) void k_d_hidden_sum(
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (d + e < width) row[d + e] = v[e];
-  }
-}
-
-// d_weight of a piece: BM columns x BN classes over the piece's rows; pieces
-// before the last add up in float32.
-template <typename TL>
-__global__ __launch_bounds__(TL::kThreads) void k_d_weight(
-    const typename TL::T *P, int64_t ldp, const typename TL::T *packed, int32_t wide,
-    int32_t vocab, int32_t width, const HeadInfo *info, int32_t piece, int32_t pieces, float *sum,
-    typename TL::T *d_weight, int64_t d_stride, int32_t vec) {
-  using T = typename TL::T;
-  __shared__ __align__(1024) char lds[TL::kLdsOut];
-  const Piece pc = piece_of(info->rows, piece, pieces);
-  const uint32_t col_tiles = (uint32_t)(width + TL::BM - 1) / TL::BM;
-  const uint32_t v_tiles = (uint32_t)(vocab + TL::BN - 1) / TL::BN;
-  const TileAt at = tile_at(xcd_order(blockIdx.x, gridDim.x), v_tiles, col_tiles);
-  const int32_t v0 = at.slow * TL::BN, d0 = at.fast * TL::BM;
-  typename TL::A a;
-  typename TL::B b;
-  a.init(packed + (int64_t)pc.begin * wide, wide, d0, wide);
-  b.init(P, ldp, v0, (int32_t)ldp);
-  Acc4 acc[TL::MI][TL::NI] = {};
-  TL::walk(a, b, 0, (pc.rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
-  if (pieces > 1) {
-    const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
-    const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
-#pragma unroll
-    for (int j = 0; j < TL::NI; ++j) {
-      const int32_t v = v0 + wn + j * 16 + (l & 15);
-      if (v >= vocab) continue;
-#pragma unroll
-      for (int i = 0; i < TL::MI; ++i) {
-        const int32_t d = d0 + wm + i * 16 + (l >> 4) * 4;
-        if (d >= wide) continue;
-        Acc4 *p = reinterpret_cast<Acc4 *>(sum + (int64_t)v * wide + d);
-        if (piece > 0) acc[i][j] += *p;
-        if (piece < pieces - 1) *p = acc[i][j];
-      }
-    }
-    if (piece < pieces - 1) return;
-  }
-  const float back = info->from_operand;
-  TL::stage_out(lds, [&](int i, int j, int r) { return (T)(acc[i][j][r] * back); });
-  __syncthreads();
-  if (vec) {
-    TL::read_out(lds, [&](int n, int m, Int4 x) {
-      if (v0 + n < vocab && d0 + m < width)
-        *reinterpret_cast<Int4 *>(d_weight + (int64_t)(v0 + n) * d_stride + d0 + m) = x;
-    });
-  } else {
-    TL::read_out_one(lds, [&](int n, int m, T x) {
-      if (v0 + n < vocab && d0 + m < width) d_weight[(int64_t)(v0 + n) * d_stride + d0 + m] = x;
-    });
   }
 }
 
@@ -760,32 +801,44 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
     const int64_t piece = std::min<int64_t>(rows, p.piece_rows);
     p.d_hidden = piece <= 32 ? kThin : !f32 && width >= 256 && piece >= 256 ? kBig : kMid;
     if (p.d_hidden == kMid && tiles_of(kMid, width, piece) < kCus / 16) p.d_hidden = kThin;
+    p.d_weight = shape(width, vocab);
     // d_hidden's sums run over the whole vocabulary, in parts that fill the
-    // CUs.  What a number of parts costs, in microseconds: rounds of tiles (a
-    // CU holds one kBig, two kMid or kThin), each with a start and an end, and
-    // the parts' sums written and read.  The rates are the kernels' own.  How
-    // many rows count is not known here: the mean over half, three quarters and
-    // all of them.
+    // CUs.  The times here, in microseconds, are the kernels' own.
     const int64_t step = 128 / es, steps = (vocab + step - 1) / step;
     const int64_t tiles = tiles_of(p.d_hidden, width, piece);
-    const int64_t at_once = p.d_hidden == kBig ? kCus : 2 * kCus;
-    const double step_us = (f32 ? 8.0 : 1.0) * (p.d_hidden == kBig ? 1.4 : p.d_hidden == kMid ? 0.8 : 0.3);
-    const double part_us = (double)piece * p.wide * 8 / 4e6;
-    double best = 0.0;
-    for (int64_t n = 1; n <= std::min<int64_t>(64, std::max<int64_t>(1, steps / 4)); ++n) {
-      double rounds = 0.0;
-      for (int64_t share = 2; share <= 4; ++share)
-        rounds += (double)((tiles * share / 4 * n + at_once - 1) / at_once) * 4 / share / 3;
-      const double us =
-          rounds * ((double)((steps + n - 1) / n) * step_us + 6.0) + (double)n * part_us;
-      if (n == 1 || us < best) {
-        best = us;
-        p.splits = (int32_t)n;
+    const int64_t most = std::min<int64_t>(64, std::max<int64_t>(1, steps / 4));
+    if (p.d_hidden == kBig && p.d_weight == kBig) {
+      // One launch with d_weight's tiles behind: as few parts as make a tile
+      // take half of the whole at most.
+      const double step_us = 1.45, whole =
+          (double)(tiles * steps) * step_us +
+          (double)tiles_of(kBig, width, vocab) * ((double)(piece + 63) / 64 * step_us + 10.0);
+      const double longest = 0.5 * whole / kCus;
+      p.splits = (int32_t)std::min<int64_t>(
+          most, std::max<int64_t>(1, (int64_t)std::ceil((double)steps * step_us / longest)));
+    } else {
+      // What a number of parts costs: rounds of tiles (a CU holds two), each with
+      // a start and an end, and the parts' sums written and read.  How many rows
+      // count is not known here: the mean over half, three quarters and all.
+      const int64_t at_once = p.d_hidden == kBig ? kCus : 2 * kCus;
+      const double step_us =
+          (f32 ? 8.0 : 1.0) * (p.d_hidden == kBig ? 1.4 : p.d_hidden == kMid ? 0.8 : 0.3);
+      const double part_us = (double)piece * p.wide * 8 / 4e6;
+      double best = 0.0;
+      for (int64_t n = 1; n <= most; ++n) {
+        double rounds = 0.0;
+        for (int64_t share = 2; share <= 4; ++share)
+          rounds += (double)((tiles * share / 4 * n + at_once - 1) / at_once) * 4 / share / 3;
+        const double us =
+            rounds * ((double)((steps + n - 1) / n) * step_us + 6.0) + (double)n * part_us;
+        if (n == 1 || us < best) {
+          best = us;
+          p.splits = (int32_t)n;
+        }
       }
     }
     p.split_v = (int32_t)((steps + p.splits - 1) / p.splits * step);
     p.splits = (int32_t)((vocab + p.split_v - 1) / p.split_v);
-    p.d_weight = shape(width, vocab);
   }
   // Loads are of 16 bytes, within 2^31 bytes of a tile's first row.
   p.pack_weight = ((uintptr_t)weight & 15) || w_stride * es % 16 || width * es % 16 ||
@@ -908,23 +961,33 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
         info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
         z_label, P, p.ldp, own_rest, c.row_loss, c.lse);
     if (!c.grad) continue;
-    by_shape<T>(p.d_hidden, [&](auto s) {
-      using TL = TileOf<T, decltype(s)::value, true, false>;
-      k_d_hidden<TL><<<(unsigned)(tiles_of(s, w_width, piece) * p.splits), TL::kThreads, 0, st>>>(P, p.ldp, weight, w_stride, p.vocab, w_width,
-                                                p.wide, info, k, p.pieces, p.splits, p.split_v,
-                                                part, part_stride);
-    });
+    const ProductArgs g{P, p.ldp, packed, p.wide, p.vocab, p.width, info, k, p.pieces, weight,
+                        w_stride, w_width, p.splits, p.split_v, part, part_stride, sum, c.d_weight,
+                        c.dw_stride, dw_vec};
+    const unsigned hidden = (unsigned)(tiles_of(p.d_hidden, w_width, piece) * p.splits);
+    const unsigned weights = (unsigned)tiles_of(p.d_weight, p.width, p.vocab);
+    bool both = false;
+    if constexpr (sizeof(T) == 2)
+      if (p.d_hidden == kBig && p.d_weight == kBig) {
+        using TH = TileOf<T, kBig, true, false>;
+        using TW = TileOf<T, kBig, true, true>;
+        const unsigned first = (hidden + 7) / 8 * 8;
+        k_products<TH, TW><<<first + weights, TH::kThreads, 0, st>>>(g, first);
+        both = true;
+      }
+    if (!both) {
+      by_shape<T>(p.d_hidden, [&](auto s) {
+        using TL = TileOf<T, decltype(s)::value, true, false>;
+        k_d_hidden<TL><<<hidden, TL::kThreads, 0, st>>>(g);
+      });
+      by_shape<T>(p.d_weight, [&](auto s) {
+        using TL = TileOf<T, decltype(s)::value, true, true>;
+        k_d_weight<TL><<<weights, TL::kThreads, 0, st>>>(g);
+      });
+    }
     k_d_hidden_sum<T><<<(unsigned)piece + 1, 256, 0, st>>>(
         k, p.pieces, loss, p.splits, part, part_stride, p.wide, p.width, lab, own_rest, weight,
         w_stride, static_cast<T *>(c.d_hidden), c.dh_stride, dh_vec);
-    by_shape<T>(p.d_weight, [&](auto s) {
-      using TL = TileOf<T, decltype(s)::value, true, true>;
-      k_d_weight<TL><<<(unsigned)tiles_of(s, p.width, 1) *
-                           (unsigned)((p.vocab + TL::BN - 1) / TL::BN),
-                       TL::kThreads, 0, st>>>(
-          P, p.ldp, packed, p.wide, p.vocab, p.width, info, k, p.pieces, sum,
-          static_cast<T *>(c.d_weight), c.dw_stride, dw_vec);
-    });
   }
   if (!c.grad) k_loss_sum<<<1, 1024, 0, st>>>(loss);
   return launched();
