@@ -338,6 +338,7 @@ int norm_and_clip(int32_t device, void *stream, int32_t count, const void *const
   DeviceScope scope;
   rc = scope.enter(device);
   if (rc != BSSCL_OK) return rc;
+  (void)hipGetLastError();  // what an earlier call left is not this one's
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto *sums = static_cast<double *>(workspace);
   int32_t n = 0;

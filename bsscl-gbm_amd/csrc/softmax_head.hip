@@ -44,8 +44,10 @@ constexpr float kExpScale = std::is_same<T, _Float16>::value ? 32768.f : 1.f;
 
 template <typename T>
 __device__ __forceinline__ T from_float(float x) {
-  if constexpr (std::is_same<T, _Float16>::value)
-    x = fminf(fmaxf(x, -65504.f), 65504.f);
+  if constexpr (std::is_same<T, _Float16>::value) {  // (a NaN stays one)
+    if (x > 65504.f) x = 65504.f;
+    if (x < -65504.f) x = -65504.f;
+  }
   return (T)x;
 }
 
@@ -1018,6 +1020,7 @@ int head(int32_t device, void *stream, int32_t dtype, int64_t rows, int64_t widt
   DeviceScope scope;
   const int drc = scope.enter(device);
   if (drc != BSSCL_OK) return drc;
+  (void)hipGetLastError();  // what an earlier call left is not this one's
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == BSSCL_BF16) return run_head<__bf16>(st, p, c);
   if (dtype == BSSCL_F16) return run_head<_Float16>(st, p, c);

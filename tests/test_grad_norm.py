@@ -83,9 +83,9 @@ def test_c_entries_refuse():
 
 # -- on the GPU ---------------------------------------------------------------
 @pytest.mark.gpu
-@pytest.mark.parametrize("sizes", [[1], [0, 3, 0], [7, 16384, 16385, 1, 40000],
+@pytest.mark.parametrize("sizes", [[1], [0], [0, 3, 0], [7, 16384, 16385, 1, 40000],
                                    [5] * 300, [1000003, 13], list(range(1, 260))],
-                         ids=["one", "empty", "edges", "many", "large", "ragged"])
+                         ids=["one", "nothing", "empty", "edges", "many", "large", "ragged"])
 @pytest.mark.parametrize("inv_scale", [1.0, -1.0 / 128])
 def test_norm_and_clip(sizes, inv_scale):
     print(f"[case] clip {len(sizes)} tensors, {sum(sizes)} values, {inv_scale}", flush=True)

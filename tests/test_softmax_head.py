@@ -121,6 +121,22 @@ def test_sizes(rows, width, vocab, dtype):
     _both(h, w, y, grad_scale=256.0 if dtype == "fp16" else 1.0)
 
 
+# Enough tiles for the largest shape, at edges of it in every axis.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("rows,width,vocab,kw", [
+    (513, 264, 40001, {}), (300, 1001, 33000, {}), (2100, 256, 12800, dict(left_out=0.4)),
+    (700, 328, 20011, dict(softcap=20.0, z_loss=1e-3, left_out=0.2)),
+    (129, 520, 70000, dict(left_out=0.1))])
+def test_large_tiles(rows, width, vocab, kw, dtype):
+    print(f"[case] head {rows} x {width} x {vocab} {kw} {dtype}", flush=True)
+    kw = dict(kw)
+    h, w, y = make(rows, width, vocab, DTYPES[dtype], seed=rows, left_out=kw.pop("left_out", 0.0))
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(1)).cuda()
+    _both(h, w, y, row_weight=u, grad_scale=512.0 if dtype == "fp16" else 1.0, **kw)
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("kw", [dict(softcap=4.0), dict(z_loss=0.01), dict(reduction="sum"),
@@ -227,6 +243,69 @@ def test_rows_in_several_pieces(dtype):
         Head(h, w, y).check(got)
         del got
         torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_wide_rows_in_several_pieces():
+    """As above with both products in one launch."""
+    print("[case] head pieces 2700 x 264 x 262147", flush=True)
+    h, w, y = make(2700, 264, 262147, torch.bfloat16, seed=4, left_out=0.1)
+    got = linear_softmax_grad(h, w, y)
+    Head(h, w, y).check(got)
+    del got
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("rows", [5, 300])
+def test_nan_stays_where_it_belongs(rows, dtype):
+    """A NaN in a counting row: its own loss and d_hidden, and all of d_weight;
+    the other rows are what they are without it."""
+    print(f"[case] head NaN {rows} {dtype}", flush=True)
+    h, w, y = make(rows, 64, 500, DTYPES[dtype], seed=17)
+    want = linear_softmax_grad(h, w, y, reduction="sum")
+    few = linear_softmax_loss(h, w, y, reduction="sum")
+    h[2, 5] = float("nan")
+    others = torch.arange(rows, device="cuda") != 2
+    got = linear_softmax_grad(h, w, y, reduction="sum")
+    for g, x in ((got, want), (linear_softmax_loss(h, w, y, reduction="sum"), few)):
+        assert bool(torch.isnan(g.loss)) and bool(torch.isnan(g.row_loss[2]))
+        assert bool(torch.isnan(g.lse[2]))
+        assert torch.equal(g.row_loss[others], x.row_loss[others])
+        assert torch.equal(g.lse[others], x.lse[others])
+    assert bool(torch.isnan(got.d_hidden[2]).all()) and bool(torch.isnan(got.d_weight).all())
+    assert torch.equal(got.d_hidden[others], want.d_hidden[others])
+
+
+@pytest.mark.gpu
+def test_one_token_without_a_batch():
+    h, w, y = make(1, 64, 300, torch.bfloat16, seed=1)
+    want = linear_softmax_grad(h, w, y)
+    got = linear_softmax_grad(h[0], w, y[0])
+    assert got.row_loss.shape == () and got.d_hidden.shape == (64,)
+    assert torch.equal(got.d_hidden, want.d_hidden[0]) and torch.equal(got.loss, want.loss)
+    score = linear_softmax_loss(h[0], w, y[0])
+    assert abs(float(score.row_loss) - float(want.row_loss)) <= 1e-5 * abs(float(want.row_loss))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls that overlap have workspaces of their own."""
+    cases = [make(400, 128, 3000, torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [linear_softmax_grad(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(linear_softmax_grad(*cases[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for g in got[k]:
+            for a, b in zip(g, want[k]):
+                assert torch.equal(a, b)
 
 
 @pytest.mark.gpu
