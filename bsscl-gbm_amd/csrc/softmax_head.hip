@@ -728,16 +728,17 @@ __global__ __launch_bounds__(256) void k_pack_weight(const T *weight, int64_t st
 }
 
 // The tile shapes: 256 x 256 fills the matrix cores best and needs a whole
-// CU's LDS; 128 x 128 gives four times the workgroups; 128 x 32 wastes less
-// where there are few rows.
+// CU's LDS; three of 128 x 64 share a CU (128 x 128 takes 461 us where it takes
+// 424, 700 x 1,024 x 30,011 float32: fewer rows are padding, and the last round
+// is shorter); 128 x 32 wastes less where there are few rows.
 enum Shape : int32_t { kBig, kMid, kThin };
 template <typename T, Shape S, bool A_ACROSS, bool B_ACROSS>
 using TileOf = std::conditional_t<
     S == kBig, Tile<T, 256, 256, 128, 64, A_ACROSS, B_ACROSS, 128, 2>,
-    std::conditional_t<S == kMid, Tile<T, 128, 128, 64, 64, A_ACROSS, B_ACROSS, 128, 2>,
+    std::conditional_t<S == kMid, Tile<T, 128, 64, 64, 32, A_ACROSS, B_ACROSS, 128, 2>,
                        Tile<T, 128, 32, 32, 32, A_ACROSS, B_ACROSS, 128, 3>>>;
 constexpr int shape_m(Shape s) { return s == kBig ? 256 : 128; }
-constexpr int shape_n(Shape s) { return s == kBig ? 256 : s == kMid ? 128 : 32; }
+constexpr int shape_n(Shape s) { return s == kBig ? 256 : s == kMid ? 64 : 32; }
 
 int64_t tiles_of(Shape s, int64_t m, int64_t n) {
   return ((m + shape_m(s) - 1) / shape_m(s)) * ((n + shape_n(s) - 1) / shape_n(s));
@@ -819,12 +820,12 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
       p.splits = (int32_t)std::min<int64_t>(
           most, std::max<int64_t>(1, (int64_t)std::ceil((double)steps * step_us / longest)));
     } else {
-      // What a number of parts costs: rounds of tiles (a CU holds two), each with
-      // a start and an end, and the parts' sums written and read.  How many rows
+      // What a number of parts costs: rounds of tiles (a CU holds three kMid or two
+      // kThin), each with a start and an end, and the parts' sums written and read.  How many rows
       // count is not known here: the mean over half, three quarters and all.
-      const int64_t at_once = p.d_hidden == kBig ? kCus : 2 * kCus;
+      const int64_t at_once = (p.d_hidden == kBig ? 1 : p.d_hidden == kMid ? 3 : 2) * kCus;
       const double step_us =
-          (f32 ? 8.0 : 1.0) * (p.d_hidden == kBig ? 1.4 : p.d_hidden == kMid ? 0.8 : 0.3);
+          (f32 ? 8.0 : 1.0) * (p.d_hidden == kBig ? 1.4 : p.d_hidden == kMid ? 0.6 : 0.3);
       const double part_us = (double)piece * p.wide * 8 / 4e6;
       double best = 0.0;
       for (int64_t n = 1; n <= most; ++n) {
