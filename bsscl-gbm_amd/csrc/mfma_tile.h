@@ -57,9 +57,10 @@ __device__ __forceinline__ Acc4 mma(Int4 a, Int4 b, Acc4 acc) {
 
 // 16 bytes per lane from memory to LDS at lds_at + 16 lane.  In assembly
 // because the compiler would wait for it before every transposing read; the
-// walk below waits itself.
+// walk below waits itself.  (A write of m0 needs a wait state before the load;
+// the compiler reserves m0 and has no use of its own for it here.)
 __device__ __forceinline__ void load_to_lds(Int4 rsrc, uint32_t offset, uint32_t lds_at) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_at), "v"(offset), "s"(rsrc)
                : "memory");
@@ -263,10 +264,15 @@ struct Tile {
             wait_and_meet<(STAGES - 2) * kLoads>();
             fa[0] = A::fragment(from, wm, np);
           }
-          if (last && i >= r0)
+          if (last && i >= r0) {
 #pragma unroll
-            for (int e = (i - r0) * kLoads / rows; e < (i - r0 + 1) * kLoads / rows; ++e)
-              if (e < A::kLoads) a.load(sa, e); else b.load(sb, e - A::kLoads);
+            for (int e = (i - r0) * kLoads / rows; e < (i - r0 + 1) * kLoads / rows; ++e) {
+              if (e < A::kLoads)
+                a.load(sa, e);
+              else
+                b.load(sb, e - A::kLoads);
+            }
+          }
           if (i >= r0)
 #pragma unroll
             for (int j = (i - r0) * NI / rows; j < (i - r0 + 1) * NI / rows; ++j)

@@ -778,10 +778,10 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
   p.vocab = (int32_t)vocab;
   // The largest tile that gives every other CU one and whose rows are not for
   // the most part padding.  Measured (us, kBig against kMid): scores of 64 rows x
-  // 4,096 x 131,072 bf16 306 and 258, of 256 rows 293 and 419, of 512 rows x
-  // 2,048 x 32,000 (250 tiles) 70 and 97; d_weight of 16 to 1,500 rows 37 and 40
-  // to 197 and 240; kMid against kThin: scores of 700 x 1,024 x 30,011 float32
-  // 458 and 473, of 128 x 512 x 4,099 (33 tiles) 48 and 18.
+  // 4,096 x 131,072 bf16 308 and 248, of 256 rows 293 and 475, of 512 rows x
+  // 2,048 x 32,000 (250 tiles) 70 and 115; d_weight of 16 rows x 2,048 x 32,000 38
+  // and 44, of 1,500 rows 187 and 291; kMid against kThin: scores of 700 x 1,024 x
+  // 30,011 float32 425 and 474, of 128 x 512 x 4,099 (66 tiles) 29 and 18.
   auto shape = [&](int64_t m, int64_t n) {
     if (!f32 && n > 128 && tiles_of(kBig, m, n) >= kCus / 2) return kBig;
     return n > 32 && tiles_of(kMid, m, n) >= kCus / 2 ? kMid : kThin;
