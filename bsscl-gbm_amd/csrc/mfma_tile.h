@@ -82,7 +82,9 @@ struct Operand {
   static constexpr int kChunks = kRowBytes / 16;  // of an LDS row
   static constexpr int kRowsPerLoad = 64 / kChunks;
   static constexpr int kLoads = kBytes / 1024 / WAVES;  // of each wave in a step
-  static_assert(kLoads >= 1 && kLoads * 1024 * WAVES == kBytes && kChunks <= 64, "tile shape");
+  static_assert(kLoads >= 1 && kLoads * 1024 * WAVES == kBytes && kChunks <= 64 &&
+                    WAVES % 2 == 0,  // (a lane then has one chunk in all its loads)
+                "tile shape");
 
   // The place of chunk c of LDS row r, its own inverse.  Banks repeat every 256
   // bytes.  Sixteen lanes read at once
