@@ -69,6 +69,11 @@ def _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, grad_s
                                    or row_weight.dtype != torch.float32
                                    or row_weight.shape != labels.shape):
         raise ValueError("row_weight must be a float32 tensor of the labels' shape")
+    for name, x in (("softcap", softcap), ("z_loss", z_loss)):
+        if not 0.0 <= x < math.inf:
+            raise ValueError(f"{name} must be finite and >= 0, got {x}")
+    if grad_scale is not None and not math.isfinite(grad_scale):
+        raise ValueError(f"grad_scale must be finite, got {grad_scale}")
     dev = hidden.device
     if dev.type != "cuda":
         raise ValueError("hidden must be on a GPU")
@@ -91,14 +96,14 @@ def _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, grad_s
         if grad:
             out[4].zero_()
         return out
-    hidden = hidden.reshape(rows, width)
+    hidden, weight = hidden.reshape(rows, width).resolve_neg(), weight.resolve_neg()
     if width > 1 and hidden.stride(1) != 1 or rows > 1 and hidden.stride(0) < width:
         hidden = hidden.contiguous()
     if width > 1 and weight.stride(1) != 1 or vocab > 1 and weight.stride(0) < width:
         weight = weight.contiguous()
-    labels = labels.reshape(rows).to(torch.int64).contiguous()
+    labels = labels.reshape(rows).resolve_neg().to(torch.int64).contiguous()
     if row_weight is not None:
-        row_weight = row_weight.reshape(rows).contiguous()
+        row_weight = row_weight.reshape(rows).resolve_neg().contiguous()
     h_stride = max(hidden.stride(0), width)  # a single row may have any stride
     w_stride = max(weight.stride(0), width)
     L = _native.lib()
@@ -205,7 +210,8 @@ def _norm(tensors, inv_scale, max_norm, out):
         out = list(out)
         outs, _, out_codes, out_index = _list(torch, out, "out")
         if len(out) != n or out_codes != codes or out_index != index or any(
-                o.shape != t.shape or o.stride() != t.stride() for o, t in zip(out, tensors)):
+                o.shape != t.shape or o.stride() != t.stride() or o.is_neg() != t.is_neg()
+                for o, t in zip(out, tensors)):
             raise ValueError("out must match tensors in number, shape, strides, dtype and GPU")
 
     def at(a):

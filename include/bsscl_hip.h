@@ -506,7 +506,7 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
  * bsscl_head_grad adds, times grad_scale,
  *   d_hidden = d loss / d hidden (rows x width, stride d_hidden_stride) and
  *   d_weight = d loss / d weight (vocab x width, stride d_weight_stride),
- * both of the inputs' dtype and overwritten.
+ * both of the inputs' dtype and overwritten.  No output may overlap an input.
  * Sums run in float32.  d loss / d score is rounded to the inputs' dtype as
  * operand of the two products, divided by the largest row weight first (so that
  * equal weights are exact); what that takes of the label's value is added to

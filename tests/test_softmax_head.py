@@ -65,10 +65,19 @@ def test_refuses_tensors_that_do_not_fit():
             ((h, w, y.float()), {}, "int64 or int32"),
             ((h, w, y), dict(reduction="none"), "reduction"),
             ((h, w, y), dict(row_weight=torch.ones(3)), "row_weight"),
-            ((h, w, y), dict(row_weight=torch.ones(4).double()), "row_weight")]:
+            ((h, w, y), dict(row_weight=torch.ones(4).double()), "row_weight"),
+            ((h, w, y), dict(softcap=-1.0), "softcap"),
+            ((h[:0], w, y[:0]), dict(softcap=float("inf")), "softcap"),
+            ((h, w, y), dict(z_loss=float("nan")), "z_loss")]:
         for fn in (linear_softmax_loss, linear_softmax_grad):
             with pytest.raises(ValueError, match=what):
                 fn(*args, **kw)
+
+
+def test_refuses_a_grad_scale_that_is_not_finite():
+    h, w, y = make(4, 8, 16, torch.float32, device="cpu")
+    with pytest.raises(ValueError, match="grad_scale"):
+        linear_softmax_grad(h, w, y, grad_scale=float("inf"))
 
 
 def test_c_entries_refuse_bad_sizes():
@@ -203,6 +212,7 @@ def test_layouts(dtype):
             "odd offset": (wide(h, 1, 2), wide(w, 3, 2), y),
             "transposed": (h.t().contiguous().t(), w.t().contiguous().t(), y),
             "labels": (h, w, strided_labels), "int32": (h, w, y.int()),
+            "negated views": (torch._neg_view(-h), torch._neg_view(-w), y),
             "batched": (h.reshape(4, 24, 64), w, y.reshape(4, 24)),
             "batch slice": (torch.cat([h.reshape(4, 24, 64)] * 2, 1)[:, :24], w,
                             y.reshape(4, 24))}.items():
