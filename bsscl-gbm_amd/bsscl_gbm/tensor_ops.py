@@ -72,6 +72,8 @@ def _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, grad_s
     for name, x in (("softcap", softcap), ("z_loss", z_loss)):
         if not 0.0 <= x < math.inf:
             raise ValueError(f"{name} must be finite and >= 0, got {x}")
+    if 0.0 < softcap < 1e-6:
+        raise ValueError(f"softcap must be 0 or at least 1e-6, got {softcap}")
     if grad_scale is not None and not math.isfinite(grad_scale):
         raise ValueError(f"grad_scale must be finite, got {grad_scale}")
     dev = hidden.device
@@ -131,7 +133,7 @@ def linear_softmax_loss(hidden, weight, labels, *, row_weight=None, reduction="m
     [0, vocab), such as -1 or -100, is left out: its loss and lse are 0,
     whatever its hidden values are.  row_weight (...) float32 weighs the rows;
     reduction "mean" divides by the counting rows' sum of weights, "sum" does
-    not.  softcap c > 0 puts c * tanh(s / c) in the place of each score, and
+    not.  softcap c >= 1e-6 puts c * tanh(s / c) in the place of each score, and
     z_loss zeta adds zeta * lse^2 to each row's loss.
 
     Returns (loss, row_loss, lse) in float32: the reduced loss, each row's

@@ -220,7 +220,9 @@ __device__ __forceinline__ TileAt tile_at(uint32_t at, uint32_t slow, uint32_t f
 
 // tanh(s / c) for to_exp = 2 log2(e) / c, off by less than 2.5 of 2^-24: as
 // 1 - 2 / (1 + e^{2 |s| / c}) the quotient is at most 1 and the exponential's
-// error counts at most half.
+// error counts at most half.  Times a cap of up to kFastCap that is 1e-5 of a
+// score at most; larger caps, of which scores are a small part, take tanhf.
+constexpr float kFastCap = 64.f;
 __device__ __forceinline__ float tanh_of(float s, float to_exp) {
   const float e = __builtin_amdgcn_exp2f(fabsf(s) * to_exp);
   return copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e), s);
@@ -274,7 +276,9 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
           acc[i][j][r] = f(acc[i][j][r], wm + i * 16 + (l >> 4) * 4 + r);
   };
   const float to_slope = softcap > 0.f ? 1.f / softcap : 0.f;
-  if (softcap > 0.f) {
+  if (softcap > kFastCap) {
+    each([&](float z, int) { return softcap * tanhf(z / softcap); });
+  } else if (softcap > 0.f) {
     const float to_exp = 2.f * kLog2E / softcap;
     each([&](float z, int) { return softcap * tanh_of(z, to_exp); });
   }
@@ -832,9 +836,10 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
       p.splits = (int32_t)std::min<int64_t>(
           most, std::max<int64_t>(1, (int64_t)std::ceil((double)steps * step_us / longest)));
     } else {
-      // What a number of parts costs: rounds of tiles (a CU holds three kMid or two
-      // kThin), each with a start and an end, and the parts' sums written and read.  How many rows
-      // count is not known here: the mean over half, three quarters and all.
+      // What a number of parts costs: rounds of tiles (a CU holds three kMid or
+      // two kThin), each with a start and an end, and the parts' sums written and
+      // read.  How many rows count is not known here: the mean over half, three
+      // quarters and all.
       const int64_t at_once = (p.d_hidden == kBig ? 1 : p.d_hidden == kMid ? 3 : 2) * kCus;
       const double step_us =
           (f32 ? 8.0 : 1.0) * (p.d_hidden == kBig ? 1.4 : p.d_hidden == kMid ? 0.6 : 0.3);
@@ -951,8 +956,8 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
     w_stride = w_width = p.wide;
   }
   const PrepareArgs prep{c.labels, c.row_weight, p.rows, p.vocab, c.mean, c.grad_scale,
-                         sizeof(T) == 4, std::is_same<T, _Float16>::value, idx, lab, u, pos, c.row_loss, c.lse,
-                         info};
+                         sizeof(T) == 4, std::is_same<T, _Float16>::value, idx, lab, u, pos,
+                         c.row_loss, c.lse, info};
   const bool count = p.rows <= kCountRows;
   if (!count) k_head_prepare<<<1, 1024, 0, st>>>(prep);
   k_pack_hidden<T><<<(unsigned)p.rows + kRowPad + (count ? 1 : 0), 256, 0, st>>>(
@@ -1021,10 +1026,11 @@ int head(int32_t device, void *stream, int32_t dtype, int64_t rows, int64_t widt
     return set_error(BSSCL_EINVAL, "softmax head: a row stride is below the width");
   if (reduction != BSSCL_SUM && reduction != BSSCL_MEAN)
     return set_error(BSSCL_EINVAL, "softmax head: unknown reduction");
-  if (!(c.softcap >= 0.f) || !std::isfinite(c.softcap) || !(c.z_loss >= 0.f) ||
-      !std::isfinite(c.z_loss) || !std::isfinite(c.grad_scale))
+  if (!(c.softcap == 0.f || (c.softcap >= 1e-6f && std::isfinite(c.softcap))))
+    return set_error(BSSCL_EINVAL, "softmax head: softcap must be 0 or finite and >= 1e-6");
+  if (!(c.z_loss >= 0.f) || !std::isfinite(c.z_loss) || !std::isfinite(c.grad_scale))
     return set_error(BSSCL_EINVAL,
-                     "softmax head: softcap and z_loss must be finite and >= 0, grad_scale finite");
+                     "softmax head: z_loss must be finite and >= 0, grad_scale finite");
   if ((size_t)workspace_bytes < p.bytes || ((uintptr_t)c.ws & 255))
     return set_error(BSSCL_EINVAL, "softmax head: the workspace holds " +
                                        std::to_string(workspace_bytes) + " of " +

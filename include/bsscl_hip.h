@@ -497,7 +497,7 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
  *   labels      int64[rows]; a row whose label is outside [0, vocab) is left
  *               out: its outputs are 0 whatever its hidden values are
  *   row_weight  float32[rows] or NULL for ones
- *   softcap     c > 0: z = c tanh(s / c) in the place of each score s; 0: none
+ *   softcap     c >= 1e-6: z = c tanh(s / c) in the place of each score s; 0: none
  *   z_loss      zeta >= 0: each row's loss gets + zeta * lse^2
  * With z the scores, lse = log sum exp z and u the row weights (reduction):
  *   row_loss[i] = lse_i - z_i[label_i] + zeta lse_i^2,   loss = sum u_i row_loss[i]

@@ -68,6 +68,7 @@ def test_refuses_tensors_that_do_not_fit():
             ((h, w, y), dict(row_weight=torch.ones(4).double()), "row_weight"),
             ((h, w, y), dict(softcap=-1.0), "softcap"),
             ((h[:0], w, y[:0]), dict(softcap=float("inf")), "softcap"),
+            ((h, w, y), dict(softcap=1e-9), "softcap"),
             ((h, w, y), dict(z_loss=float("nan")), "z_loss")]:
         for fn in (linear_softmax_loss, linear_softmax_grad):
             with pytest.raises(ValueError, match=what):
@@ -100,7 +101,7 @@ def test_c_entries_refuse_bad_sizes():
                                  fake, fake, fake, ws_ptr, ws_bytes)
 
     for kw in [dict(ws_bytes=16), dict(h=None), dict(hs=7), dict(ws_ptr=ctypes.c_void_p(4100)),
-               dict(red=2), dict(cap=-1.0), dict(cap=float("nan")), dict(zl=-0.1),
+               dict(red=2), dict(cap=-1.0), dict(cap=1e-9), dict(cap=float("inf")), dict(cap=float("nan")), dict(zl=-0.1),
                dict(zl=float("inf"))]:
         assert loss(**kw) == _native.BSSCL_EINVAL, kw
 
@@ -238,6 +239,29 @@ def test_large_scores():
     _both(h, w, y)
     h, w, y = make(70, 64, 300, torch.bfloat16, seed=2, spread=600.0)
     _both(h, w, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [9, 200])
+def test_caps_far_above_the_scores_change_nothing(rows):
+    """c tanh(s / c) = s - s^3 / (3 c^2) + ...: 4e-6 at c = 10,000 for scores of
+    11; rounding adds 2 steps of 2^-24 of tanh's relative error and as much for
+    the quotient and the product, 4e-6 together."""
+    h, w, y = make(rows, 64, 700, torch.float32, seed=12, spread=2.0)
+    assert float((h @ w.T).abs().max()) < 20
+    plain = linear_softmax_loss(h, w, y, reduction="sum")
+    most = float((h @ w.T).abs().max())
+    capped = linear_softmax_loss(h, w, y, reduction="sum", softcap=1e4)
+    tol = most ** 3 / 3e8 * 1.1 + 12 * 2.0 ** -24 * most
+    assert float((plain.lse - capped.lse).abs().max()) <= tol
+    assert float((plain.row_loss - capped.row_loss).abs().max()) <= 2 * tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-3, 64.0, 65.0, 1000.0])
+def test_caps(cap):
+    h, w, y = make(150, 72, 900, torch.float32, seed=13, spread=5.0, left_out=0.2)
+    _both(h, w, y, softcap=cap)
 
 
 @pytest.mark.gpu
