@@ -218,14 +218,18 @@ __device__ __forceinline__ TileAt tile_at(uint32_t at, uint32_t slow, uint32_t f
   return {(int32_t)(in / width), (int32_t)(group * kGroup + in % width)};
 }
 
-// tanh(s / c) for to_exp = 2 log2(e) / c, off by less than 2.5 of 2^-24: as
-// 1 - 2 / (1 + e^{2 |s| / c}) the quotient is at most 1 and the exponential's
-// error counts at most half.  Times a cap of up to kFastCap that is 1e-5 of a
-// score at most; larger caps, of which scores are a small part, take tanhf.
-constexpr float kFastCap = 64.f;
-__device__ __forceinline__ float tanh_of(float s, float to_exp) {
-  const float e = __builtin_amdgcn_exp2f(fabsf(s) * to_exp);
-  return copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e), s);
+// tanh(x), off by less than 6e-7 of itself: from 0.3 on 1 - 2 / (1 + e^{2 |x|}),
+// whose error is less than 2.5 of 2^-24 (the quotient is at most 1 and the
+// exponential's error counts at most half), and below that the series, whose
+// first term left out is 6e-8 of it.  Relative, so that a cap far above the
+// scores leaves them as they are.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float e = __builtin_amdgcn_exp2f(fabsf(x) * (2.f * kLog2E)), q = x * x;
+  float t = fmaf(q, 62.f / 2835.f, -17.f / 315.f);
+  t = fmaf(q, t, 2.f / 15.f);
+  t = fmaf(q, t, -1.f / 3.f);
+  t = fmaf(q * x, t, x);
+  return fabsf(x) < 0.3f ? t : copysignf(1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e), x);
 }
 
 // Score tiles: BM classes x BN rows.  Label: int32 for packed rows, int64 for
@@ -276,12 +280,7 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
           acc[i][j][r] = f(acc[i][j][r], wm + i * 16 + (l >> 4) * 4 + r);
   };
   const float to_slope = softcap > 0.f ? 1.f / softcap : 0.f;
-  if (softcap > kFastCap) {
-    each([&](float z, int) { return softcap * tanhf(z / softcap); });
-  } else if (softcap > 0.f) {
-    const float to_exp = 2.f * kLog2E / softcap;
-    each([&](float z, int) { return softcap * tanh_of(z, to_exp); });
-  }
+  if (softcap > 0.f) each([&](float z, int) { return softcap * tanh_of(z * to_slope); });
   if (v0 + TL::BM > vocab)
     each([&](float z, int v) { return v0 + v < vocab ? z : -INFINITY; });
   // A lane holds rows wn + 16 j + l % 16 and four classes of each 16; the lanes
