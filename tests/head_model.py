@@ -4,7 +4,7 @@ the kernels may be from them, from the roundings that they make.
 Roundings counted, with u the half step of the inputs' dtype and
 e = 2^-24 that of float32:
   scores    sums of `width` exact products in float32: at most
-            (width + 2) e sum_k |h_k W_vk|; tanhf under a cap: 4 e cap more
+            (width + 2) e sum_k |h_k W_vk|; tanh under a cap: 4 e cap more
   exp, sum  expf and logf to 4 e; at most 512 additions follow each other
             within a tile and between tiles
   d score   rounded to the dtype twice (the exponential, then the normalised
