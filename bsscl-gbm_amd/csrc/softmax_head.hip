@@ -238,7 +238,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 // Classes are the m of the tile, so that a lane holds 4 MI classes of each of
 // its rows and a row's maximum and sum take two lane exchanges and, where two
 // waves share it, one through LDS.  With many rows the matrix cores are the
-// bound (6,144 x 4,096 x 131,072 bf16 5.4 ms, 1.2 PFLOP/s with 1.6 GB of
+// bound (6,144 x 4,096 x 131,072 bf16 5.3 ms, 1.25 PFLOP/s with 1.6 GB of
 // exponentials written), and the tile's end costs 10 to 17 us; with few rows the
 // weight's bytes are (1 x 2,048 x 32,000 bf16 22 us, 6 TB/s from the caches).
 template <typename TL, typename Label>
