@@ -159,18 +159,12 @@ def prepare(case, seed):
     return dict(case, grads=grads, out=out)
 
 
-_pkg = None
-
-
 def _package():
-    """The package, imported once, as a program does."""
-    global _pkg
-    if _pkg is None:
-        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-        sys.path.insert(0, os.path.join(root, "bsscl-gbm_amd"))
-        import bsscl_gbm
-        _pkg = bsscl_gbm
-    return _pkg
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bsscl-gbm_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import bsscl_gbm
+    return bsscl_gbm
 
 
 def _run_own(s):
