@@ -370,7 +370,8 @@ __device__ __forceinline__ float wave_add(float v) {
 }
 
 // (m, s) with s exp(m) the sum over the tiles first, first + by, ...: rescaled
-// as the maximum grows.
+// as the maximum grows.  (A tile of maximum -inf holds no score above it: its sum
+// is 0, or NaN, which stays.)
 __device__ __forceinline__ float2 tiles_sum(const float2 *st, int32_t tiles, int32_t first,
                                             int32_t by) {
   float m = -INFINITY, s = 0.f;
@@ -378,10 +379,10 @@ __device__ __forceinline__ float2 tiles_sum(const float2 *st, int32_t tiles, int
   for (int32_t t = first; t < tiles; t += by) {
     const float2 x = st[t];
     if (x.x > m) {
-      s = m == -INFINITY ? x.y : s * expf(m - x.x) + x.y;
+      s = m == -INFINITY ? s + x.y : s * expf(m - x.x) + x.y;
       m = x.x;
     } else {
-      s += x.x == -INFINITY ? x.y : x.y * expf(x.x - m);  // (NaN stays NaN)
+      s += x.x == -INFINITY ? x.y : x.y * expf(x.x - m);
     }
   }
   return make_float2(m, s);
