@@ -8,7 +8,7 @@
 //   m = max m_t,   lse = m + log sum_t s_t exp(m_t - m).
 // For the gradient a tile also leaves exp(z - m_t) (times the cap's slope) in
 // the inputs' dtype: k_rows turns it into d loss / d score by one factor per
-// row and tile, exp(m_t - lse) times the row's weight, and puts the label's
+// row and tile, exp(m_t - m) / s times the row's weight, and puts the label's
 // own value there from its float32 score, where p - 1 keeps what a rounded p
 // would lose.  These rows of the vocabulary's length are made for a piece of
 // the rows at a time (kPieceBytes), and both products consume a piece before
@@ -318,13 +318,15 @@ __global__ __launch_bounds__(TL::kThreads) void k_scores(
   }
 #pragma unroll
   for (int j = 0; j < TL::NI; ++j) {
-    const float base = top[j] == -INFINITY ? 0.f : -top[j] * kLog2E;
+    // The difference first: the maximum's exponential is 1 whatever its size, so
+    // that sums are at least 1 and no p exceeds 1.
+    const float base = top[j] == -INFINITY ? 0.f : top[j];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < TL::MI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = acc[i][j][r], e = __builtin_amdgcn_exp2f(fmaf(z, kLog2E, base));
+        const float z = acc[i][j][r], e = __builtin_amdgcn_exp2f((z - base) * kLog2E);
         s += e;
         if (!P) continue;
         if (softcap > 0.f) {
@@ -388,9 +390,20 @@ __device__ __forceinline__ float2 tiles_sum(const float2 *st, int32_t tiles, int
   return make_float2(m, s);
 }
 
-// lse of a row from its tiles' statistics, by the block's kRowThreads threads.
+// (m, s) of a row from its tiles' statistics: lse = m + log s.
+__device__ __forceinline__ float lse_of(float2 x) {
+  return (x.x == -INFINITY ? 0.f : x.x) + logf(x.y);
+}
+// The row's negative log-probability of its label, whose score is zy: the parts
+// of lse apart, so that a loss far below lse keeps its digits and none is
+// below 0 (zy is one of the scores, and s is at least 1).
+__device__ __forceinline__ float minus_log_p(float2 x, float zy) {
+  return ((x.x == -INFINITY ? 0.f : x.x) - zy) + logf(x.y);
+}
+
+// A row's (m, s) by the block's kRowThreads threads.
 constexpr int kRowThreads = 256;
-__device__ float row_lse(const float2 *st, int32_t tiles, float *red) {
+__device__ float2 row_sum(const float2 *st, int32_t tiles, float *red) {
   constexpr int kWaves = kRowThreads / 64;
   const int tid = (int)threadIdx.x, wid = tid >> 6;
   const float2 own = tiles_sum(st, tiles, tid, kRowThreads);
@@ -408,7 +421,7 @@ __device__ float row_lse(const float2 *st, int32_t tiles, float *red) {
   s = red[kWaves];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) s += red[kWaves + w];
-  return (top == -INFINITY ? 0.f : top) + logf(s);
+  return make_float2(top, s);
 }
 
 // Up to kFewRows rows as the caller has them, one block: each wave takes a part
@@ -434,10 +447,10 @@ __global__ __launch_bounds__(1024) void k_few_rows(const int64_t *labels, const 
   const int r = (int)threadIdx.x;
   if (r < rows) {
     const float2 x = tiles_sum(part[r], parts, 0, 1);
-    const float lse = (x.x == -INFINITY ? 0.f : x.x) + logf(x.y);
+    const float lse = lse_of(x);
     const int64_t y = labels[r];
     const bool counts = y >= 0 && y < vocab;
-    const float l = counts ? lse - z_label[r] + z_loss * lse * lse : 0.f;
+    const float l = counts ? minus_log_p(x, z_label[r]) + z_loss * lse * lse : 0.f;
     row_loss[r] = l;
     lse_out[r] = counts ? lse : 0.f;
     value[r] = l;
@@ -478,22 +491,22 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
     return;
   }
   const float2 *st = stats + (int64_t)r * tiles;
-  const float lse = row_lse(st, tiles, red);
+  const float2 sum = row_sum(st, tiles, red);
   const int32_t c = pc.begin + r, y = lab[c];
-  const float zy = z_label[r];
+  const float zy = z_label[r], lse = lse_of(sum), nll = minus_log_p(sum, zy);
   if (tid == 0) {
-    row_loss[idx[c]] = lse - zy + z_loss * lse * lse;
+    row_loss[idx[c]] = nll + z_loss * lse * lse;
     lse_out[idx[c]] = lse;
   }
   if (!P) return;
   const float g = u[c] * grad_scale * info->to_operand, zl = 2.f * z_loss * lse;
-  const float py = expm1f(zy - lse);
+  const float py = expm1f(-nll);
   const float slope = softcap > 0.f ? 1.f - (zy / softcap) * (zy / softcap) : 1.f;
   const float own = g * slope * (py + zl * (py + 1.f));
   // What rounding takes of the label's value, the row's largest as a rule:
   // k_d_hidden_sum adds it times the label's row of the weight.
   if (tid == 0) own_rest[r] = own - (float)from_float<T>(own);
-  const float scale = g * (1.f + zl) / kExpScale<T>;
+  const float scale = g * (1.f + zl) / (kExpScale<T> * sum.y);
   const int tile_shift = 31 - __clz(tile_v / kVec);
   for (int32_t i0 = tid; i0 < n; i0 += kRowThreads * kVecs) {
     Int4 x[kVecs];
@@ -510,7 +523,7 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
     for (int k = 0; k < kVecs; ++k) {
       const int32_t i = i0 + k * kRowThreads;
       if (i >= n) continue;
-      const float by = expf(f[k] - lse) * scale;
+      const float by = expf(f[k] - sum.x) * scale;
       typedef T TV __attribute__((ext_vector_type(kVec)));
       TV v = __builtin_bit_cast(TV, x[k]);
 #pragma unroll

@@ -27,6 +27,68 @@ def picked(rows, vocab, tops, gap, dtype=torch.float32):
     return h.to(dtype).cuda(), w.cuda(), y.cuda()
 
 
+# -- rows that are nearly certain, scores of any size -----------------------
+TOPS = [t + k / 16 for k in range(16) for t in (10, 13, 23, 27, 46, 57, 90, 120)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [32, 384])
+def test_nearly_certain_rows(rows):
+    """No loss below 0 and no p above 1 where the other classes lie 12 to 24
+    below the label (or 10 to 127, those at 0), and losses as fine as float32
+    sums near 1 allow.
+
+    The scores are exact.  A tile's sum and those of all tiles take at most 64
+    additions to a value in [1, 2), each off by 2^-24, logf and expm1f 4 of
+    2^-24 of less than 1: 72 e.  The other classes' p are exponentials of at
+    most 24, whose difference and product with log2 e are rounded once each and
+    whose constant is off by half as much: 60 e, and 36 e for the exponential,
+    the sum and the factors."""
+    print(f"[case] head nearly certain {rows}", flush=True)
+    h, w, y = picked(rows, 640, TOPS, 12.0)
+    z = torch.cat([h.double(), torch.zeros(rows, 576, dtype=torch.float64, device="cuda")], 1)
+    at = torch.arange(rows, device="cuda")
+    rest = z - z[at, y][:, None]
+    rest[at, y] = -math.inf
+    loss = torch.log1p(rest.exp().sum(1))
+    got = linear_softmax_grad(h, w, y, reduction="sum")
+    for r in (linear_softmax_loss(h, w, y, reduction="sum"), got):
+        assert float(r.row_loss.min()) >= 0
+        assert float((r.row_loss.double() - loss).abs().max()) <= 72 * E
+    ds = torch.exp(rest - loss[:, None])[:, :64]
+    ds[at, y] = torch.expm1(-loss)
+    assert float(got.d_hidden[at, y].max()) <= 0
+    off = (got.d_hidden.double() - ds).abs()
+    tol = 96 * E * ds.abs() + 1e-44
+    tol[at, y] = 72 * E
+    assert bool((off <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [5, 40])
+@pytest.mark.parametrize("top", [-3e4, 1e6, -3e9, 1e10, 1e30])
+def test_scores_of_any_size(top, rows):
+    """Only differences to the maximum are exponentials, whatever it is: 63
+    classes lie far below the label, which is certain if its score is above 0
+    and (with 576 classes at 0) has no mass otherwise."""
+    print(f"[case] head scores {top} {rows}", flush=True)
+    for dtype in [torch.float32, torch.bfloat16] + ([torch.float16] if abs(top) < 6e4 else []):
+        h, w, y = picked(rows, 640, [top], abs(top) / 4, dtype)
+        at = torch.arange(rows, device="cuda")
+        top_y = h.double()[at, y]
+        want = torch.zeros(rows, dtype=torch.float64, device="cuda") if top > 0 else \
+            math.log(576) - top_y
+        got = linear_softmax_grad(h, w, y, reduction="sum")
+        for r in (linear_softmax_loss(h, w, y, reduction="sum"), got):
+            assert float((r.row_loss.double() - want).abs().max()) <= 4 * E * float(want.max())
+            lse = top_y if top > 0 else torch.full_like(top_y, math.log(576))
+            assert float((r.lse.double() - lse).abs().max()) <= 4 * E * float(lse.abs().max())
+        ds = torch.zeros_like(got.d_hidden)
+        if top < 0:
+            ds[at, y] = -1
+        assert torch.equal(got.d_hidden, ds)
+
+
 # -- NaN in whole tiles ------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,vocab,classes", [(1, 9000, 8192), (9, 8500, 128), (3, 40000, 20000),
