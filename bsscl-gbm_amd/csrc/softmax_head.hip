@@ -35,21 +35,34 @@ struct HeadInfo {
   int32_t rows;      // counting rows
   float to_operand;  // what d loss / d score is multiplied by as an operand
   float from_operand;
+  float lift;        // of the piece: its operands are divided by it as well
+  int32_t low, high;  // in_order of the finite tile maxima so far (float16 with z-loss)
 };
+
+// Integers in the order of floats, its own inverse (for atomic minima and maxima).
+__device__ __forceinline__ int32_t in_order(int32_t bits) {
+  return bits ^ ((bits >> 31) & 0x7fffffff);
+}
+
+// Float16 operands hold 1 + 2 zeta lse up to 32 (63, with what the label's value
+// adds); beyond that a power of two is divided out.  lse lies between the row's
+// maximum, itself no lower than the lowest tile's, and the highest plus log of the
+// classes, which is known before the piece's rows are scaled.
+__device__ __forceinline__ float lift_of(const HeadInfo *info, float z_loss, float log_classes) {
+  const float low = __builtin_bit_cast(float, in_order(info->low));
+  const float high = __builtin_bit_cast(float, in_order(info->high));
+  const float most = fmaxf(fabsf(1.f + 2.f * z_loss * low),
+                           fabsf(1.f + 2.f * z_loss * (high + log_classes)));
+  if (!(most > 32.f && most < INFINITY)) return 1.f;
+  int e;
+  (void)frexpf(most / 32.f, &e);
+  return ldexpf(1.f, e);
+}
 
 // A tile's exponentials, at most 1, are kept times this: in float16 they would
 // lose digits below 2^-14 of the tile's maximum otherwise.
 template <typename T>
 constexpr float kExpScale = std::is_same<T, _Float16>::value ? 32768.f : 1.f;
-
-template <typename T>
-__device__ __forceinline__ T from_float(float x) {
-  if constexpr (std::is_same<T, _Float16>::value) {  // (a NaN stays one)
-    if (x > 65504.f) x = 65504.f;
-    if (x < -65504.f) x = -65504.f;
-  }
-  return (T)x;
-}
 
 int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
@@ -147,14 +160,17 @@ __device__ void prepare(const PrepareArgs &a, double *tmp) {
     // are given) then have d loss / d label score at p - 1, which bf16 and
     // float16 hold to p for surprising labels, and not off by half a step like
     // any other multiple.  In float16 it becomes 2^10: a factor of 2^5 and more
-    // is left to the largest value (1 + 2 zeta lse may exceed 1), and the
-    // smallest lies at 2^-35 of the weight.
+    // is left to the largest value (1 + 2 zeta lse may exceed 1; lift_of), and
+    // the smallest lies at 2^-35 of the weight.
     float m = (float)(big * fabs(share)) * fabsf(a.grad_scale);
     if (!(m >= 0x1p-100f && m <= 0x1p100f)) m = 1.f;
     const float one = a.narrow ? 1024.f : 1.f;
     a.info->rows = base;
     a.info->to_operand = a.whole ? 1.f : one / m;
     a.info->from_operand = a.whole ? 1.f : m / one;
+    a.info->lift = 1.f;
+    a.info->low = in_order(__builtin_bit_cast(int32_t, INFINITY));
+    a.info->high = in_order(__builtin_bit_cast(int32_t, -INFINITY));
   }
   if (a.mean)
     for (int32_t p = tid; p < base; p += THREADS) a.u[p] = (float)((double)a.u[p] * share);
@@ -467,13 +483,37 @@ __global__ __launch_bounds__(1024) void k_few_rows(const int64_t *labels, const 
   *loss = (float)(!mean ? s : all != 0.0 ? s / all : 0.0);
 }
 
+// The range of a piece's finite tile maxima, joined to that of the pieces before
+// it.  A pass of its own over what the tiles left, with one pair of atomics a
+// block (7 us of 600 at 1,500 x 32,003; 15 with a pair a wave, and a pair at the
+// end of each wave of a tile made the tiles take 55 us longer there).
+constexpr int kRangeBlocks = 64;
+__global__ __launch_bounds__(1024) void k_range(HeadInfo *info, int32_t piece, int32_t pieces,
+                                                int32_t tiles, const float2 *stats) {
+  __shared__ float tmp[1024];
+  const int64_t n = (int64_t)piece_of(info->rows, piece, pieces).rows * tiles;
+  float low = INFINITY, high = -INFINITY;
+#pragma unroll 4
+  for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n; i += kRangeBlocks * 1024) {
+    const float top = stats[i].x;
+    const bool finite = fabsf(top) < INFINITY;
+    low = fminf(low, finite ? top : INFINITY);
+    high = fmaxf(high, finite ? top : -INFINITY);
+  }
+  low = block_fold<1024>(low, tmp, [](float x, float y) { return fminf(x, y); });
+  high = block_fold<1024>(high, tmp, [](float x, float y) { return fmaxf(x, y); });
+  if (threadIdx.x != 0) return;
+  atomicMin(&info->low, in_order(__builtin_bit_cast(int32_t, low)));
+  atomicMax(&info->high, in_order(__builtin_bit_cast(int32_t, high)));
+}
+
 // One block per row of the piece: lse and loss from the tiles' statistics;
 // with P, the row of d loss / d score in its place.  Bound by memory with P: a
 // block keeps kVecs 16-byte loads a thread in flight (6,144 x 131,072 bf16 read
 // and written in 600 us, 5.4 TB/s; 645 us with loads that stay in the caches).
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void k_rows(
-    const HeadInfo *info, int32_t piece, int32_t pieces, const int32_t *idx, const int32_t *lab,
+    HeadInfo *info, int32_t piece, int32_t pieces, const int32_t *idx, const int32_t *lab,
     const float *u, float softcap, float z_loss, float grad_scale, int32_t tiles, int32_t tile_v,
     const float2 *stats, const float *z_label, T *P, int64_t ldp, float *own_rest,
     float *row_loss, float *lse_out) {
@@ -499,13 +539,19 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
     lse_out[idx[c]] = lse;
   }
   if (!P) return;
-  const float g = u[c] * grad_scale * info->to_operand, zl = 2.f * z_loss * lse;
+  float lift = 1.f;
+  if constexpr (std::is_same<T, _Float16>::value)
+    if (z_loss > 0.f) {
+      lift = lift_of(info, z_loss, logf((float)ldp));
+      if (r == 0 && tid == 0) info->lift = lift;  // for the products
+    }
+  const float g = u[c] * grad_scale * (info->to_operand / lift), zl = 2.f * z_loss * lse;
   const float py = expm1f(-nll);
   const float slope = softcap > 0.f ? 1.f - (zy / softcap) * (zy / softcap) : 1.f;
   const float own = g * slope * (py + zl * (py + 1.f));
   // What rounding takes of the label's value, the row's largest as a rule:
   // k_d_hidden_sum adds it times the label's row of the weight.
-  if (tid == 0) own_rest[r] = own - (float)from_float<T>(own);
+  if (tid == 0) own_rest[r] = own - (float)(T)own;
   const float scale = g * (1.f + zl) / (kExpScale<T> * sum.y);
   const int tile_shift = 31 - __clz(tile_v / kVec);
   for (int32_t i0 = tid; i0 < n; i0 += kRowThreads * kVecs) {
@@ -528,7 +574,7 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
       TV v = __builtin_bit_cast(TV, x[k]);
 #pragma unroll
       for (int e = 0; e < kVec; ++e)
-        v[e] = from_float<T>(i * kVec + e == y ? own : (float)v[e] * by);
+        v[e] = (T)(i * kVec + e == y ? own : (float)v[e] * by);
       row[i] = __builtin_bit_cast(Int4, v);
     }
   }
@@ -611,6 +657,7 @@ __device__ __forceinline__ void d_weight_tile(const ProductArgs &g, uint32_t blo
   b.init(static_cast<const T *>(g.P), g.ldp, v0, (int32_t)g.ldp);
   Acc4 acc[TL::MI][TL::NI] = {};
   TL::walk(a, b, 0, (pc.rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
+  const float lift = g.info->lift;
   if (pieces > 1) {
     const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
     const int wm = wave / TL::kWavesN * TL::WM, wn = wave % TL::kWavesN * TL::WN;
@@ -623,13 +670,14 @@ __device__ __forceinline__ void d_weight_tile(const ProductArgs &g, uint32_t blo
         const int32_t d = d0 + wm + i * 16 + (l >> 4) * 4;
         if (d >= wide) continue;
         Acc4 *p = reinterpret_cast<Acc4 *>(g.sum + (int64_t)v * wide + d);
+        acc[i][j] *= lift;
         if (piece > 0) acc[i][j] += *p;
         if (piece < pieces - 1) *p = acc[i][j];
       }
     }
     if (piece < pieces - 1) return;
   }
-  const float back = g.info->from_operand;
+  const float back = pieces > 1 ? g.info->from_operand : g.info->from_operand * lift;
   TL::stage_out(lds, [&](int i, int j, int r) { return (T)(acc[i][j][r] * back); });
   __syncthreads();
   if (g.dw_vec) {
@@ -706,7 +754,7 @@ __global__ __launch_bounds__(256) void k_d_hidden_sum(
   const Piece pc = piece_of(info->rows, piece, pieces);
   const int32_t r = (int32_t)blockIdx.x - 1;
   if (r >= pc.rows) return;
-  const float back = info->from_operand;
+  const float back = info->from_operand * info->lift;
   T *row = d_hidden + (int64_t)loss.idx[pc.begin + r] * d_stride;
   const T *own_row = weight + (int64_t)lab[pc.begin + r] * w_stride;
   const float rest = own_rest[r];
@@ -990,6 +1038,9 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
           weight, w_stride, p.vocab, w_width, packed, p.wide, lab, info, k, p.pieces, c.softcap,
           p.tiles, stats, z_label, P, p.ldp);
     });
+    if constexpr (std::is_same<T, _Float16>::value)
+      if (c.grad && c.z_loss > 0.f)
+        k_range<<<kRangeBlocks, 1024, 0, st>>>(info, k, p.pieces, p.tiles, stats);
     k_rows<T><<<(unsigned)(c.grad ? p.piece_rows : piece), kRowThreads, 0, st>>>(
         info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
         z_label, P, p.ldp, own_rest, c.row_loss, c.lse);

@@ -511,7 +511,9 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
  * operand of the two products, divided by the largest row weight first (so that
  * equal weights are exact); what that takes of the label's value is added to
  * d_hidden again.  In float16 it holds at least 2^-35 of the largest row
- * weight, and 1 + 2 zeta lse may reach 32.
+ * weight; where 1 + 2 zeta lse may exceed 32 in either sign, 2^-39 of that
+ * weight times the largest such value (lse taken from the lowest maximum of 128
+ * or 256 classes to the highest score plus log vocab).
  * 1 <= rows <= 8000000, 1 <= width <= 65536, 1 <= vocab <= 4000000.
  */
 int bsscl_head_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t vocab,

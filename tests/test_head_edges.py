@@ -104,3 +104,67 @@ def test_nan_in_whole_tiles_of_classes(rows, vocab, classes):
         for r in (linear_softmax_loss(h, w, y), linear_softmax_grad(h, w, y)):
             assert bool(torch.isnan(r.loss))
             assert bool(torch.isnan(r.row_loss).all()) and bool(torch.isnan(r.lse).all())
+
+
+# -- a strong z-loss in float16 ----------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("factor", [20.0, 63.0, 81.0, 200.0, 600.0])
+@pytest.mark.parametrize("rows,vocab", [(48, 700), (700, 33000)])
+def test_strong_z_loss_in_float16(factor, rows, vocab):
+    """1 + 2 zeta lse far above 1, with most of the mass on another class than
+    the label.  The operand's scale then falls by as much (to the next power of
+    two, and log(vocab) may be in the bound of lse twice over): its half step
+    2^-35 grows by at most 4 factor / 32."""
+    print(f"[case] head z-loss {factor} {rows} x {vocab}", flush=True)
+    h, w, y = make(rows, 72, vocab, torch.float16, seed=3, spread=1.0, left_out=0.1)
+    h = (h.float() + 40.0 * w[(y + 1) % vocab].float()).half()
+    lse = torch.logsumexp(h.double() @ w.double().T, 1)[y >= 0]
+    zeta = (factor - 1) / (2 * float(lse.median()))
+    u = torch.linspace(0.25, 1.0, rows).cuda()
+    m = Head(h, w, y, row_weight=u, z_loss=zeta, reduction="sum")
+    more = float(u.max()) * 2.0 ** -35 * 4 * max(1.0, factor * float(lse.max() / lse.median()) / 32)
+    m.tol_d_hidden += more * m.w.abs().sum(0)
+    m.tol_d_weight += more * m.h.abs().sum(0)
+    m.check(linear_softmax_grad(h, w, y, row_weight=u, z_loss=zeta, reduction="sum"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeta", [0.5, 30.0])
+def test_strong_z_loss_below_zero_in_float16(zeta):
+    """lse far below 0: 1 + 2 zeta lse far below -1.  (Head takes the factor's
+    sign into the exponentials' share of a tolerance: twice the share's size
+    gives it back.)"""
+    print(f"[case] head z-loss {zeta}, lse below 0", flush=True)
+    h, w, y = make(300, 64, 200, torch.float16, seed=4, spread=1.0)
+    h[:, 0], w[:, 0] = -8.0, 8.0  # every score 64 lower
+    m = Head(h, w, y, z_loss=zeta)
+    assert float(m.lse.max()) < -40
+    f = (1 + 2 * zeta * m.lse).abs()[:, None]
+    err = 66 * E * (m.h.abs() @ m.w.abs().T).amax(1, keepdim=True)
+    e_exp = 3 * err + 664 * E + 4 * E * m.lse.abs()[:, None]
+    p = torch.exp(m.h @ m.w.T - m.lse[:, None])
+    back = 2 * f * e_exp / 300 * (p + torch.zeros_like(p).scatter_(1, y[:, None], 1.0))
+    more = 2.0 ** -35 * 4 * float(f.max()) / 32 / 300
+    m.tol_d_hidden += more * m.w.abs().sum(0) + back @ m.w.abs()
+    m.tol_d_weight += more * m.h.abs().sum(0) + back.T @ m.h.abs()
+    m.check(linear_softmax_grad(h, w, y, z_loss=zeta))
+
+
+@pytest.mark.gpu
+def test_strong_z_loss_in_several_pieces_in_float16():
+    """Each piece has an operand scale of its own; lse rises from piece to
+    piece, and the sums over pieces are of the same unit."""
+    rows, vocab = 600, 1_100_003
+    print(f"[case] head z-loss pieces {rows} x 8 x {vocab}", flush=True)
+    h, w, y = make(rows, 8, vocab, torch.float16, seed=4)
+    h = (h.float() * torch.linspace(0.2, 6.0, rows).cuda()[:, None]).half()
+    kw = dict(z_loss=4.0, reduction="sum", grad_scale=1 / 16)
+    m = Head(h, w, y, **kw)
+    f = float((1 + 8 * m.lse).abs().max())
+    assert f > 100
+    more = 2.0 ** -35 * 4 * f / 32 / 16
+    m.tol_d_hidden += more * m.w.abs().sum(0)
+    m.tol_d_weight += more * m.h.abs().sum(0)
+    m.check(linear_softmax_grad(h, w, y, **kw))
+    del m
+    torch.cuda.empty_cache()
