@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void k_scale(const ClipList list, const d
       constexpr int N = 16 / (int)sizeof(T), kBatch = 8;
       const T *x = static_cast<const T *>(list.from[at.t]);
       T *o = static_cast<T *>(list.to[at.t]);
-      if (fa == 1.f && x == o) return;
+      if (fa == 1.f && !small && x == o) return;
       const bool whole = (((uintptr_t)x ^ (uintptr_t)o) & 15) == 0;
       x -= at.lead;
       o -= at.lead;

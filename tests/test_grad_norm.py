@@ -227,3 +227,16 @@ def test_training_step_with_the_head(dtype):
         check(before, grads, norm, max_norm, 1.0 / scale)
         assert norm64(grads) <= max_norm * (1 + 2 * half_step(dtype))
         w = (w.float() - 2.0 * grads[1].float()).to(dtype)
+
+
+@pytest.mark.gpu
+def test_factors_next_to_the_smallest_normal_float32():
+    """Factors that are 1 but for a power of two scale all the same."""
+    x = torch.linspace(1.0, 2.0, 1000, device="cuda")
+    for inv_scale in (2.0 ** -126, math.nextafter(2.0 ** -126, 0.0), 2.0 ** -127):
+        t, o = x.clone(), torch.empty_like(x)
+        clip_grads([t], 1.0, inv_scale=inv_scale)
+        clip_grads([x], 1.0, inv_scale=inv_scale, out=[o])
+        assert torch.equal(t, o)
+        exact = x.double() * inv_scale
+        assert bool(((t.double() - exact).abs() <= 2.0 ** -149).all())
