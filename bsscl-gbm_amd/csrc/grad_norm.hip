@@ -331,8 +331,8 @@ int norm_and_clip(int32_t device, void *stream, int32_t count, const void *const
   int rc = sums_of(count, lengths, &most);
   if (rc == BSSCL_OK) rc = check_list(count, tensors, out, lengths, dtypes);
   if (rc != BSSCL_OK) return rc;
-  if (!std::isfinite(inv_scale))
-    return set_error(BSSCL_EINVAL, "gradient norm: inv_scale must be finite");
+  if (!std::isfinite((float)inv_scale))  // (an infinite factor would make zeros NaN)
+    return set_error(BSSCL_EINVAL, "gradient norm: inv_scale must be finite in float32");
   if (!norm || !workspace || ((uintptr_t)workspace & 255) ||
       workspace_bytes < most * (int64_t)sizeof(double))
     return set_error(BSSCL_EINVAL,

@@ -537,10 +537,10 @@ int bsscl_head_grad(int32_t device, void *stream, int32_t dtype, const void *hid
  * dtypes in host arrays), and the tensors scaled to it:
  *   norm = |inv_scale| sqrt(sum of squares)            (float32[1])
  *   out[t][i] = tensors[t][i] * inv_scale * min(1, max_norm / norm)
- * Squares are summed in float64 in a fixed order.  A norm that is NaN or
- * infinite clips nothing (the factor is inv_scale): the caller sees it in
- * `norm`.  out[t] may be tensors[t] itself; otherwise no out may overlap any
- * tensor, and no two outs may overlap (refused).
+ * Squares are summed in float64 in a fixed order.  inv_scale has to be finite
+ * in float32.  A norm that is NaN or infinite clips nothing (the factor is
+ * inv_scale): the caller sees it in `norm`.  out[t] may be tensors[t] itself;
+ * otherwise no out may overlap any tensor, and no two outs may overlap (refused).
  */
 int bsscl_grad_norm_workspace(int32_t count, const int64_t *lengths, int64_t *bytes);
 int bsscl_grad_norm(int32_t device, void *stream, int32_t count, const void *const *tensors,

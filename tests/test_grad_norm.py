@@ -240,3 +240,17 @@ def test_factors_next_to_the_smallest_normal_float32():
         assert torch.equal(t, o)
         exact = x.double() * inv_scale
         assert bool(((t.double() - exact).abs() <= 2.0 ** -149).all())
+
+
+def test_refuses_an_inv_scale_beyond_float32():
+    """A factor that float32 holds as infinite would turn zeros into NaN."""
+    L = _native.lib()
+    norm, ws = ctypes.c_void_p(0x30000), ctypes.c_void_p(0x40000)
+    at = (ctypes.c_void_p * 1)(0x10000)
+    length, code = (ctypes.c_int64 * 1)(100), (ctypes.c_int32 * 1)(2)
+    for inv in (1e39, -1e39, 3.5e38):
+        assert L.bsscl_clip_grads(0, None, 1, at, at, length, code, inv, 1.0, norm, ws,
+                                  1 << 20) == _native.BSSCL_EINVAL
+        assert L.bsscl_grad_norm(0, None, 1, at, length, code, inv, norm, ws,
+                                 1 << 20) == _native.BSSCL_EINVAL
+        assert b"inv_scale" in L.bsscl_last_error()
