@@ -7,7 +7,8 @@ outputs are torch tensors on one GPU; the kernels are libbsscl_hip.so's
 (``bsscl_head_*``, ``bsscl_grad_norm``, ``bsscl_clip_grads`` in
 include/bsscl_hip.h) and run on torch's current stream of that GPU.  Calls
 return without waiting for the GPU and can be captured into a HIP graph.
-Nothing is recorded for autograd: gradients are what the calls return.
+Nothing is recorded for autograd: gradients are what the calls return.  A loss
+of inputs that require gradients says so when backward reaches it.
 """
 from __future__ import annotations
 
@@ -25,6 +26,7 @@ SoftmaxGrad = namedtuple("SoftmaxGrad", "loss row_loss lse d_hidden d_weight")
 
 _REDUCTIONS = {"sum": 0, "mean": 1}  # BSSCL_SUM, BSSCL_MEAN
 _dtype_codes = None
+_no_backward = None
 
 
 def _torch():
@@ -34,6 +36,37 @@ def _torch():
     if _dtype_codes is None:
         _dtype_codes = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
     return torch
+
+
+def _without_graph(torch, call, inputs):
+    """call(), whose results raise an error in backward and forward mode if an
+    input requires gradients or has a tangent: they would be missed silently."""
+    global _no_backward
+    forward_ad = torch.autograd.forward_ad
+    inputs = [t for t in inputs if isinstance(t, torch.Tensor)]
+    for t in inputs:
+        if (t.requires_grad and torch.is_grad_enabled()
+                or forward_ad.unpack_dual(t).tangent is not None):
+            break
+    else:
+        return call()
+    if _no_backward is None:
+        class NoBackward(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, call, *inputs):
+                return tuple(call())
+
+            @staticmethod
+            def backward(ctx, *grads):
+                raise RuntimeError("linear_softmax_loss records nothing for autograd: "
+                                   "linear_softmax_grad returns the gradient")
+
+            @staticmethod
+            def jvp(ctx, *tangents):
+                raise RuntimeError("linear_softmax_loss has no forward mode")
+
+        _no_backward = NoBackward
+    return _no_backward.apply(call, *inputs)
 
 
 def _stream(torch, device):
@@ -138,9 +171,13 @@ def linear_softmax_loss(hidden, weight, labels, *, row_weight=None, reduction="m
 
     Returns (loss, row_loss, lse) in float32: the reduced loss, each row's
     unweighted loss (for z_loss=0 the negative log-probability of its label)
-    and each row's log of the sum of exponentials.
+    and each row's log of the sum of exponentials.  Where an input requires
+    gradients, backward through the results raises an error: take
+    linear_softmax_grad.
     """
-    return SoftmaxLoss(*_head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, None))
+    return SoftmaxLoss(*_without_graph(
+        _torch(), lambda: _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, None),
+        (hidden, weight, row_weight)))
 
 
 def linear_softmax_grad(hidden, weight, labels, *, row_weight=None, reduction="mean", softcap=0.0,
@@ -150,7 +187,9 @@ def linear_softmax_grad(hidden, weight, labels, *, row_weight=None, reduction="m
 
     d_hidden and d_weight are the gradients of the reduced loss times
     grad_scale (the loss scale of a float16 run; clip_grads and grad_norm take
-    its inverse), in the inputs' dtype; rows left out have zeros.
+    its inverse), in the inputs' dtype; rows left out have zeros.  All results
+    are values without a graph, also where inputs require gradients: hand
+    d_hidden on with hidden.backward(r.d_hidden).
     """
     return SoftmaxGrad(*_head(hidden, weight, labels, row_weight, reduction, softcap, z_loss,
                               float(grad_scale)))

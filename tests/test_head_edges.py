@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from bsscl_gbm import linear_softmax_grad, linear_softmax_loss  # noqa: E402
+from bsscl_gbm import linear_softmax_grad, linear_softmax_loss, tensor_ops  # noqa: E402
 from head_model import E, Head, half_step  # noqa: E402
 from test_softmax_head import DTYPES, make  # noqa: E402
 
@@ -168,3 +168,52 @@ def test_strong_z_loss_in_several_pieces_in_float16():
     m.check(linear_softmax_grad(h, w, y, **kw))
     del m
     torch.cuda.empty_cache()
+
+
+# -- autograd ---------------------------------------------------------------------
+def _needs_grad(h, w, u):
+    return [(h.clone().requires_grad_(), w, u), (h, w.clone().requires_grad_(), u),
+            (h, w, u.clone().requires_grad_())]
+
+
+def check_no_backward(h, w, y, u):
+    want = linear_softmax_loss(h, w, y, row_weight=u)
+    for h2, w2, u2 in _needs_grad(h, w, u):
+        got = linear_softmax_loss(h2, w2, y, row_weight=u2)
+        leaf = torch.ones((), device=h.device, requires_grad=True)
+        for a, b in zip(got, want):
+            assert a.requires_grad and torch.equal(a, b) and float(a.detach().sum()) == float(b.sum())
+            with pytest.raises(RuntimeError, match="linear_softmax_grad"):
+                (a.sum() + leaf).backward()
+        with torch.no_grad():
+            assert not linear_softmax_loss(h2, w2, y, row_weight=u2).loss.requires_grad
+    assert not any(t.requires_grad for t in want)
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(h, torch.ones_like(h))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            linear_softmax_loss(dual, w, y)
+        assert not linear_softmax_loss(h, w, y).loss.requires_grad
+
+
+def test_a_missing_backward_is_said(monkeypatch):
+    """The same outputs, by a stand-in for the kernels' call."""
+    h, w, y = make(6, 8, 20, torch.float32, device="cpu")
+
+    def head(hidden, weight, labels, row_weight, *options):
+        row = (hidden.detach() @ weight.detach().T).logsumexp(1)
+        return [row.sum(), row, row.clone()]
+
+    monkeypatch.setattr(tensor_ops, "_head", head)
+    check_no_backward(h, w, y, torch.ones(6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [6, 50])
+def test_a_missing_backward_is_said_on_the_gpu(rows):
+    h, w, y = make(rows, 64, 300, torch.float32)
+    check_no_backward(h, w, y, torch.ones(rows).cuda())
+    got = linear_softmax_grad(h.requires_grad_(), w.requires_grad_(), y)
+    assert not any(t.requires_grad for t in got)
+    h.backward(got.d_hidden)
+    assert torch.equal(h.grad, got.d_hidden)
