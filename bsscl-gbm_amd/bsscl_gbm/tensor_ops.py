@@ -16,6 +16,7 @@ import ctypes
 import math
 from array import array
 from collections import namedtuple
+from operator import attrgetter
 
 from . import _native
 
@@ -25,6 +26,7 @@ SoftmaxLoss = namedtuple("SoftmaxLoss", "loss row_loss lse")
 SoftmaxGrad = namedtuple("SoftmaxGrad", "loss row_loss lse d_hidden d_weight")
 
 _REDUCTIONS = {"sum": 0, "mean": 1}  # BSSCL_SUM, BSSCL_MEAN
+_requires_grad = attrgetter("requires_grad")
 _dtype_codes = None
 _no_backward = None
 
@@ -258,6 +260,10 @@ def _norm(tensors, inv_scale, max_norm, out):
     def at(a):
         return a.buffer_info()[0]
 
+    written = () if max_norm is None else tensors if out is None else out
+    if torch.is_grad_enabled() and any(map(_requires_grad, written)):
+        raise ValueError("clip_grads writes to tensors that require gradients (parameters in the "
+                         "place of their gradients?): detach them or call it under no_grad")
     dev = torch.device("cuda", index)
     L = _native.lib()
     ws = _workspace(torch, dev, L.bsscl_grad_norm_workspace, n, at(lengths))
@@ -287,7 +293,8 @@ def clip_grads(tensors, max_norm, *, inv_scale=1.0, out=None):
 
     A norm that is NaN or infinite clips nothing (the factor is inv_scale):
     look at the returned norm and skip the step.  Tensors to be written may
-    not overlap each other or another tensor."""
+    not overlap each other or another tensor, nor, while gradients are
+    recorded, require gradients."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")

@@ -254,3 +254,21 @@ def test_refuses_an_inv_scale_beyond_float32():
         assert L.bsscl_grad_norm(0, None, 1, at, length, code, inv, norm, ws,
                                  1 << 20) == _native.BSSCL_EINVAL
         assert b"inv_scale" in L.bsscl_last_error()
+
+
+@pytest.mark.gpu
+def test_refuses_to_write_tensors_that_require_gradients():
+    """model.parameters() in the place of their gradients, for one."""
+    x = torch.ones(100, device="cuda")
+    p = torch.nn.Parameter(x.clone())
+    for args, kw in ((([p], 1.0), {}), (([x, p], 1.0), {}), (([p * 2], 1.0), {}),
+                     (([x], 1.0), dict(out=[p]))):
+        with pytest.raises(ValueError, match="require gradients"):
+            clip_grads(*args, **kw)
+        assert bool((p == 1).all()) and bool((x == 1).all())
+    assert float(grad_norm([p])) == 10.0  # reading is fine
+    clip_grads([p], 1.0, out=[x])
+    assert float(x[0]) == pytest.approx(0.1)
+    with torch.no_grad():
+        clip_grads([p], 1.0)
+    assert float(p.detach()[0]) == pytest.approx(0.1)
