@@ -276,6 +276,8 @@ def _norm(tensors, inv_scale, max_norm, out):
         _native.check(L.bsscl_clip_grads(*args, at(outs), at(lengths), at(codes),
                                          float(inv_scale), max_norm, norm.data_ptr(),
                                          ws.data_ptr(), ws.numel()))
+        # (So that a graph that saved one of them says so in backward.)
+        torch.autograd.graph.increment_version(written)
     return norm
 
 

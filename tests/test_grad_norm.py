@@ -272,3 +272,24 @@ def test_refuses_to_write_tensors_that_require_gradients():
     with torch.no_grad():
         clip_grads([p], 1.0)
     assert float(p.detach()[0]) == pytest.approx(0.1)
+
+
+@pytest.mark.gpu
+def test_tensors_saved_for_backward_are_known_to_be_written():
+    for into_out in (False, True):
+        x, o = torch.ones(100, device="cuda"), torch.zeros(100, device="cuda")
+        w = torch.ones(100, device="cuda", requires_grad=True)
+        written = o if into_out else x
+        loss = (w * written).sum()  # saves it
+        before = (x._version, o._version)
+        clip_grads([x], 1.0, out=[o] if into_out else None)
+        assert written._version == before[into_out] + 1
+        assert (o, x)[into_out]._version == before[not into_out]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        t = torch.ones(100, device="cuda")
+        clip_grads([t], 1.0)
+    assert float(t[0]) == pytest.approx(0.1)
+    clip_grads([t], 0.5)  # an inference tensor counts no versions
+    assert float(t[0]) == pytest.approx(0.05)
