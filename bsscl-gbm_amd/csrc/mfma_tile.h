@@ -207,7 +207,7 @@ struct Tile {
   static constexpr int kStep = A::kStep, kParts = STEP / 64;
   static constexpr int kStage = A::kBytes + B::kBytes;
   static constexpr int kLds = STAGES * kStage;
-  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && MI >= 2, "tile shape");
+  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && MI >= 2 && kParts % 2 == 0, "tile shape");
 
   // acc[mi][ni] += products of k in [k_begin, k_end); k_begin is a multiple of
   // kStep.  Every thread of the workgroup calls it; LDS is free at its end.
@@ -247,9 +247,7 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < MI; ++i) fa[i] = A::fragment(lds, wm + i * 16, 0);
     int buf = 0;
-    // SET: the half of fb that holds the step's first part.
-    auto one_step = [&](int64_t k, auto first_set) {
-      constexpr int SET = decltype(first_set)::value;
+    for (int64_t k = k_begin; k < k_end; k += kStep) {
       const int next = buf + 1 == STAGES ? 0 : buf + 1;
       const char *cur = lds + buf * kStage, *then = lds + next * kStage;
       const uint32_t at = lds_at + (uint32_t)(buf * kStage);
@@ -258,7 +256,7 @@ struct Tile {
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
         const bool last = part == kParts - 1;
-        const int set = (SET + part) & 1;
+        const int set = part & 1;  // (the step's parts are even in number)
         const char *from = last ? then : cur;
         const int np = last ? 0 : part + 1;
         // Rows of blocks beside which reads and loads are issued.
@@ -289,18 +287,7 @@ struct Tile {
           if (i >= r0) fa[i] = A::fragment(from, wm + i * 16, np);
         }
       }
-      buf = next;
-    };
-    // Steps of one part go by two, so that fb's halves stay where they are;
-    // loads and products beyond k_end are of zeros.
-    if constexpr (kParts & 1) {
-      for (int64_t k = k_begin; k < k_end; k += 2 * kStep) {
-        one_step(k, std::integral_constant<int, 0>());
-        one_step(k + kStep, std::integral_constant<int, 1>());
-      }
-    } else {
-      for (int64_t k = k_begin; k < k_end; k += kStep)
-        one_step(k, std::integral_constant<int, 0>());
+      buf = next;  // (Loads beyond k_end are of zeros.)
     }
     __builtin_amdgcn_sched_barrier(0);
     wait_and_meet<0>();
