@@ -57,10 +57,13 @@ __device__ __forceinline__ Acc4 mma(Int4 a, Int4 b, Acc4 acc) {
 
 // 16 bytes per lane from memory to LDS at lds_at + 16 lane.  In assembly
 // because the compiler would wait for it before every transposing read; the
-// walk below waits itself.  (A write of m0 needs a wait state before the load;
-// the compiler reserves m0 and has no use of its own for it here.)
+// walk below waits itself.  The compiler sees no load here and inserts no wait
+// states: one after the write of m0 (which it reserves and has no use of its own
+// for), and five after a vector instruction that wrote a register of rsrc.  The
+// move and four of s_nop are these five, whatever stands before them (up to 1% of
+// the products; with s_nop 0 they depended on what the compiler put there).
 __device__ __forceinline__ void load_to_lds(Int4 rsrc, uint32_t offset, uint32_t lds_at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds_at), "v"(offset), "s"(rsrc)
                : "memory");

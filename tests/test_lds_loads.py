@@ -96,3 +96,11 @@ def test_loads_to_lds_have_their_wait_states(tmp_path):
     assert loads > 100, "the kernels hold no loads to LDS"
     faults = [f for c in functions for f in _faults(c)]
     assert not faults, faults[:5]
+
+
+def test_each_load_brings_its_wait_states_along():
+    """Whatever the compiler puts before a load: the move to m0 and the s_nop
+    between them are the five states by themselves."""
+    with open(os.path.join(_build.CSRC, "mfma_tile.h")) as f:
+        found = re.findall(r's_mov_b32 m0, %0\\n\\ts_nop (\d+)\\n\\tbuffer_load\w+ .* lds"', f.read())
+    assert found and all(1 + int(n) + 1 >= WANTED for n in found)
