@@ -151,6 +151,25 @@ def test_strong_z_loss_below_zero_in_float16(zeta):
 
 
 @pytest.mark.gpu
+def test_strong_z_loss_in_replayed_graphs():
+    """The range of a call's scores is its own: inputs that shrink from replay
+    to replay have the gradients of eager calls."""
+    print("[case] head z-loss graph", flush=True)
+    h, w, y = make(300, 64, 700, torch.float16, seed=9, spread=4.0)
+    start = h.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = linear_softmax_grad(h, w, y, z_loss=20.0, grad_scale=1 / 16)
+    for k in (4.0, 1.0, 0.25, 2.0):
+        h.copy_(start * k)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, linear_softmax_grad(h, w, y, z_loss=20.0, grad_scale=1 / 16)):
+            assert bool(torch.isfinite(b).all()) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_strong_z_loss_in_several_pieces_in_float16():
     """Each piece has an operand scale of its own; lse rises from piece to
     piece, and the sums over pieces are of the same unit."""
@@ -168,6 +187,178 @@ def test_strong_z_loss_in_several_pieces_in_float16():
     m.check(linear_softmax_grad(h, w, y, **kw))
     del m
     torch.cuda.empty_cache()
+
+
+# -- few rows over many tiles -------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("vocab", [8193, 33000, 140001])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33])
+def test_few_rows_over_many_tiles(rows, vocab, dtype):
+    """Every division of a row's tiles among waves, several tiles a lane."""
+    print(f"[case] head few rows {rows} x {vocab} {dtype}", flush=True)
+    h, w, y = make(rows, 64, vocab, DTYPES[dtype], seed=rows)
+    u = torch.linspace(-0.5, 2.0, rows).cuda() if rows > 1 else None
+    if rows > 2:
+        y[1] = (-100, vocab, 1 << 40)[rows % 3]
+        h[1] = float("nan")
+    for kw in (dict(), dict(reduction="sum", z_loss=0.01, softcap=6.0)):
+        Head(h, w, y, row_weight=u, **kw).check(linear_softmax_loss(h, w, y, row_weight=u, **kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 8, 32])
+def test_few_rows_that_weigh_nothing(rows):
+    h, w, y = make(rows, 64, 9000, torch.bfloat16, seed=rows)
+    u = torch.tensor([1.5, -1.5] * (rows // 2)).cuda()
+    got = linear_softmax_loss(h, w, y, row_weight=u)
+    assert float(got.loss) == 0 and float(got.row_loss.min()) > 0
+    y[:] = -1
+    for reduction in ("mean", "sum"):
+        got = linear_softmax_loss(h, w, y, row_weight=u, reduction=reduction)
+        assert all(not t.any() for t in got)
+
+
+# -- the ends of the sizes ------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("rows,width,vocab", [(40, 65536, 300), (7, 65536, 129), (33, 40001, 70)])
+def test_wide_rows(rows, width, vocab, dtype):
+    """64 columns spread over wide rows of zeros, in small numbers whose scores
+    are exact: the losses have the narrow rows' bits, the gradients lie within
+    two tolerances of theirs (the sums' order differs) and are 0 elsewhere."""
+    print(f"[case] head wide {rows} x {width} x {vocab} {dtype}", flush=True)
+    t = DTYPES[dtype]
+    g = torch.Generator().manual_seed(width + rows)
+    at = torch.cat([torch.randperm(width - 66, generator=g)[:61] + 65,
+                    torch.tensor([0, 64, width - 1])]).cuda()
+    h = (torch.randint(-3, 4, (rows, 64), generator=g) / 4).to(t).cuda()
+    w = (torch.randint(-3, 4, (vocab, 64), generator=g) / 4).to(t).cuda()
+    y = torch.randint(-5, vocab, (rows,), generator=g).cuda()
+    h_wide, w_wide = (torch.zeros(len(x), width, dtype=t, device="cuda") for x in (h, w))
+    h_wide[:, at], w_wide[:, at] = h, w
+    m = Head(h, w, y)
+    want, got = linear_softmax_grad(h, w, y), linear_softmax_grad(h_wide, w_wide, y)
+    m.check(want)
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a, b)
+    for a, b, tol in ((got.d_hidden, want.d_hidden, m.tol_d_hidden),
+                      (got.d_weight, want.d_weight, m.tol_d_weight)):
+        assert bool(((a[:, at].double() - b.double()).abs() <= 2 * tol).all())
+        a[:, at] = 0
+        assert not a.any()
+    few, narrow = linear_softmax_loss(h_wide, w_wide, y), linear_softmax_loss(h, w, y)
+    m.check(narrow)
+    m.check(few)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_more_rows_than_a_piece_holds(dtype):
+    """2^20 rows and more are scored in two pieces, with a small vocabulary."""
+    rows = (1 << 20) + 777
+    print(f"[case] head {rows} rows {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    h = torch.randn(rows, 8, generator=g, device="cuda").to(DTYPES[dtype])
+    w = torch.randn(50, 8, generator=g, device="cuda").to(DTYPES[dtype])
+    y = torch.randint(-10, 50, (rows,), generator=g, device="cuda")
+    y[: rows // 50] = -1
+    m = Head(h, w, y)
+    m.check(linear_softmax_loss(h, w, y))
+    m.check(linear_softmax_grad(h, w, y))
+    y[:] = torch.randint(0, 50, (rows,), generator=g, device="cuda")
+    m = Head(h, w, y)
+    m.check(linear_softmax_loss(h, w, y))
+    m.check(linear_softmax_grad(h, w, y))
+
+
+@pytest.mark.gpu
+def test_loss_in_several_pieces_of_a_large_vocabulary():
+    """40,000 rows x 1.1 million classes take two pieces for their statistics;
+    rows scored by themselves (one piece) have the same values."""
+    print("[case] head loss pieces 40000 x 8 x 1100003", flush=True)
+    h, w, y = make(40000, 8, 1_100_003, torch.bfloat16, seed=5, left_out=0.1)
+    got = linear_softmax_loss(h, w, y, reduction="sum")
+    for a in (0, 20000, 35000, 39700):
+        Head_part = Head(h[a:a + 300], w, y[a:a + 300], reduction="sum")
+        part = linear_softmax_loss(h[a:a + 300], w, y[a:a + 300], reduction="sum")
+        Head_part.check(part)
+        assert bool(((got.row_loss[a:a + 300] - part.row_loss).abs()
+                     <= 2 * Head_part.tol_row_loss).all())
+        assert bool(((got.lse[a:a + 300] - part.lse).abs() <= 2 * Head_part.tol_lse).all())
+        del Head_part
+    total = float(got.row_loss.double().sum())
+    assert abs(float(got.loss) - total) <= 4 * E * total
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_rows_of_the_weight_megabytes_apart(dtype):
+    """Rows too far apart for the tiles' 32-bit offsets."""
+    print(f"[case] head rows of the weight apart {dtype}", flush=True)
+    h, w, y = make(50, 64, 9, DTYPES[dtype], seed=6)
+    want = linear_softmax_grad(h, w, y)
+    stride = (1 << 31) // 256 // w.element_size() + 8
+    far = torch.empty(9 * stride, dtype=w.dtype, device="cuda").as_strided((9, 64), (stride, 1))
+    far.copy_(w)
+    for a, b in zip(linear_softmax_grad(h, far, y), want):
+        assert torch.equal(a, b)
+    got = linear_softmax_loss(h[:3], far, y[:3])
+    assert torch.equal(got.row_loss, linear_softmax_grad(h[:3], w, y[:3]).row_loss)
+
+
+# -- the label's value ----------------------------------------------------------
+def label_share(got, exact, along, own):
+    """Root mean square over rows of the relative error that all of a row's
+    columns share along `along`: what the label's value is off by, since the
+    other errors differ from column to column."""
+    err = got.double() - exact
+    return float((((err * along).sum(1) / (along * along).sum(1) / own) ** 2).mean().sqrt())
+
+
+@pytest.mark.parametrize("rest,ok", [(1.0, True), (0.0, False), (-1.0, False)])
+def test_label_share_sees_the_label_s_rounding(rest, ok):
+    """A label's value rounded to bfloat16 (8 bits), with its rest added,
+    forgotten or subtracted."""
+    g = torch.Generator().manual_seed(2)
+    along = torch.randn(100, 1024, generator=g, dtype=torch.float64)
+    own = -(0.3 + 0.7 * torch.rand(100, generator=g, dtype=torch.float64))
+    held = own.bfloat16().double()
+    got = ((held + rest * (own - held))[:, None] * along).bfloat16()
+    share = label_share(got, own[:, None] * along, along, own)
+    assert (share <= 0.1 * half_step(torch.bfloat16)) == ok
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_label_s_value_is_not_rounded(dtype):
+    """Surprising labels (p < 1e-3) of unequal weights: d_hidden has the
+    label's value from float32; d_weight, with equal weights, has p - 1 to p or
+    to the half step below 1.  What rounds the outputs (half a step, independent
+    from column to column) leaves sqrt(3 / 1024) of 0.58 half steps in the share,
+    rounding p the same times p; the label's own rounding would be about 0.4."""
+    print(f"[case] head label's value {dtype}", flush=True)
+    t = DTYPES[dtype]
+    rows, width, vocab = 200, 1024, 5000
+    g = torch.Generator().manual_seed(14)
+    w = (torch.randn(vocab, width, generator=g) / 16).to(t).cuda()
+    h = torch.randn(rows, width, generator=g).to(t).cuda()
+    y = torch.randperm(vocab, generator=g)[:rows].cuda()
+    u = (0.3 + 0.7 * torch.rand(rows, generator=g)).cuda()
+    for weight in (u, None):
+        m = Head(h, w, y, row_weight=weight, reduction="sum")
+        p = torch.exp(-m.row_loss)
+        some = p < 1e-3
+        assert int(some.sum()) > 100
+        got = linear_softmax_grad(h, w, y, row_weight=weight, reduction="sum")
+        own = (p - 1) * (1 if weight is None else weight.double())
+        share = label_share(got.d_hidden[some], m.d_hidden[some], m.w[y[some]], own[some])
+        assert share <= 0.1 * half_step(t)
+        if weight is None:
+            share = label_share(got.d_weight[y[some]], m.d_weight[y[some]], m.h[some], own[some])
+            kept = torch.clamp(p[some], max=half_step(t) / 2).square().mean().sqrt()
+            assert share <= 0.1 * half_step(t) + float(kept)
 
 
 # -- autograd ---------------------------------------------------------------------
