@@ -161,7 +161,9 @@ def _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, grad_s
 def linear_softmax_loss(hidden, weight, labels, *, row_weight=None, reduction="mean", softcap=0.0,
                         z_loss=0.0):
     """Softmax cross entropy of the scores hidden @ weight.T, without keeping
-    the scores.
+    the scores: what a call takes besides its outputs is a copy of the rows with
+    a label and 8 bytes a row and 128 or 256 classes (and a copy of a weight
+    whose rows are not of 16-byte multiples).
 
     hidden (..., width) and weight (vocab, width) are bfloat16, float16 or
     float32; labels (...) int64 or int32.  A row whose label is outside
@@ -192,6 +194,10 @@ def linear_softmax_grad(hidden, weight, labels, *, row_weight=None, reduction="m
     its inverse), in the inputs' dtype; rows left out have zeros.  All results
     are values without a graph, also where inputs require gradients: hand
     d_hidden on with hidden.backward(r.d_hidden).
+
+    While it runs, a call takes room for exponentials of the scores in the
+    inputs' dtype: of all rows up to about 1 GiB + vocab * width * 4 bytes, of 1
+    GiB of rows at a time beyond that, with float32 sums of d_weight then.
     """
     return SoftmaxGrad(*_head(hidden, weight, labels, row_weight, reduction, softcap, z_loss,
                               float(grad_scale)))

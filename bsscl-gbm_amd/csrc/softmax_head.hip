@@ -11,8 +11,9 @@
 // row and tile, exp(m_t - m) / s times the row's weight, and puts the label's
 // own value there from its float32 score, where p - 1 keeps what a rounded p
 // would lose.  These rows of the vocabulary's length are made for a piece of
-// the rows at a time (kPieceBytes), and both products consume a piece before
-// the next one takes its place.
+// the rows at a time (kPieceBytes; smaller calls are one piece, whose
+// exponentials are rows x vocab in the inputs' dtype), and both products consume
+// a piece before the next one takes its place.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -184,8 +185,10 @@ __global__ __launch_bounds__(1024) void k_head_prepare(const PrepareArgs a) {
 // Block b < rows: row b to its place among the counting rows, widened with
 // zeros to `wide`, or zeros into d_hidden.  The kRowPad blocks after them: zero
 // rows up to the next multiple of kRowPad.  Up to kCountRows rows a block counts
-// its place itself, and one block more does the work of k_head_prepare: a
-// launch less (5 us of 57 at 128 x 512 x 4,099).
+// its place itself, reading the labels before its own, and one block more does the
+// work of k_head_prepare: a launch less (5 us of 57 at 128 x 512 x 4,099).  The
+// kernels' own times, in one launch and in two: 3.4 and 6.6 us for 128 rows of 512,
+// 5.5 and 7.9 for 1,024, 9.9 and 10.1 for 2,048, 20 and 15 for 4,096.
 constexpr int kCountRows = 2048;
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack_hidden(const T *hidden, int64_t stride,
@@ -255,8 +258,11 @@ __device__ __forceinline__ float tanh_of(float x) {
 // its rows and a row's maximum and sum take two lane exchanges and, where two
 // waves share it, one through LDS.  With many rows the matrix cores are the
 // bound (6,144 x 4,096 x 131,072 bf16 5.3 ms, 1.25 PFLOP/s with 1.6 GB of
-// exponentials written), and the tile's end costs 10 to 17 us; with few rows the
-// weight's bytes are (1 x 2,048 x 32,000 bf16 22 us, 6 TB/s from the caches).
+// exponentials written).  A tile's start and end cost 10 us, with a cap 19, and
+// writing the exponentials 1 to 16 more (1,536 rows x 32,768 classes bf16, three
+// rounds of tiles: 22, 33, 60 and 122 us a round at widths 512 to 4,096, with
+// exponentials 23, 49, 74 and 128).  With few rows the weight's bytes are the
+// bound (1 x 2,048 x 32,000 bf16 22 us, 6 TB/s from the caches).
 template <typename TL, typename Label>
 __global__ __launch_bounds__(TL::kThreads) void k_scores(
     const typename TL::T *weight, int64_t w_stride, int32_t vocab, int32_t width,
@@ -882,8 +888,13 @@ int head_plan(int32_t dtype, int64_t rows, int64_t width, int64_t vocab, const v
     p.d_hidden = piece <= 32 ? kThin : !f32 && width >= 256 && piece >= 256 ? kBig : kMid;
     if (p.d_hidden == kMid && tiles_of(kMid, width, piece) < kCus / 16) p.d_hidden = kThin;
     p.d_weight = shape(width, vocab);
-    // d_hidden's sums run over the whole vocabulary, in parts that fill the
-    // CUs.  The times here, in microseconds, are the kernels' own.
+    // d_hidden's sums run over the whole vocabulary, in parts that fill the CUs.
+    // The times here are estimates in microseconds; what they lead to, against half
+    // and twice the parts (products and sums of parts): 423 (468, 454) at 1,500 x
+    // 2,048 x 32,003 fp16, 474 (438, 508) at 2,047 x 1,001 x 50,257 bf16, 50 (83, 69)
+    // at 4,096 x 1,024 x 3,000 bf16, 37 (47, 34) at 2,048 x 512 x 4,099 bf16; d_hidden
+    // alone 261 (225, 305) at 64 x 4,096 x 131,072 bf16, 32 (28, 42) at 16 x 2,048 x
+    // 32,000 bf16, 1,570 (1,570, 1,610) at 1,024 x 2,048 x 50,257 float32.
     const int64_t step = 128 / es, steps = (vocab + step - 1) / step;
     const int64_t tiles = tiles_of(p.d_hidden, width, piece);
     const int64_t most = std::min<int64_t>(64, std::max<int64_t>(1, steps / 4));

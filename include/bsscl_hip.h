@@ -491,7 +491,9 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
 
 /*
  * Softmax cross entropy of scores hidden x weight^T, in tiles: no score is
- * ever written.
+ * ever written.  bsscl_head_grad's workspace holds exponentials of the scores in
+ * the inputs' dtype, of as many rows at a time as take 1 GiB (256 at least; 1 GiB +
+ * vocab x width x 4 bytes, if that is all of them), and float32 parts of d_hidden.
  *   hidden      rows x width, row stride hidden_stride (elements)
  *   weight      vocab x width, row stride weight_stride, of the same dtype
  *   labels      int64[rows]; a row whose label is outside [0, vocab) is left
