@@ -208,12 +208,21 @@ struct Tile {
   using A = Operand<T, BM, A_ACROSS, kWaves, STEP>;
   using B = Operand<T, BN, B_ACROSS, kWaves, STEP>;
   static constexpr int kStep = A::kStep, kParts = STEP / 64;
+  static constexpr int kJoin = !A_ACROSS && MI * NI <= 8 ? 4 : 0;  // steps of a sum; 0: all
   static constexpr int kStage = A::kBytes + B::kBytes;
   static constexpr int kLds = STAGES * kStage;
   static_assert(kLds <= 160 * 1024 && STAGES >= 2 && MI >= 2 && kParts % 2 == 0, "tile shape");
 
-  // acc[mi][ni] += products of k in [k_begin, k_end); k_begin is a multiple of
+  // total[mi][ni] += products of k in [k_begin, k_end); k_begin is a multiple of
   // kStep.  Every thread of the workgroup calls it; LDS is free at its end.
+  //
+  // Score tiles with registers left add up kJoin steps by themselves (128 float32
+  // terms, 256 of 16 bits) and those sums then: in one chain, 65,536 equal float32
+  // terms were off by 3e-4 of their sum, and the losses of 200 rows of 8,192 by
+  // 1.1e-6, now 1e-7 (times level: 420 us against 424, 700 x 1,024 x 30,011).  256 x
+  // 256 tiles have none left; their terms are of 16 bits, 32 to a link.  The
+  // products' chains are level with those of plain products, and joins took 10% of
+  // them (1,024 x 2,048 x 50,257 float32).
   //
   // Fragments are read one part ahead of the products that use them: a row of
   // blocks done, its A fragment of the next part is read in its place.  A step
@@ -228,7 +237,7 @@ struct Tile {
   // reads in front of the products it was 1.15, and with steps of half the bytes
   // in four or five buffers 1.2 (k contiguous: half lines, twice the requests).
   __device__ static __forceinline__ void walk(const A &a, const B &b, int64_t k_begin,
-                                              int64_t k_end, char *lds, Acc4 (&acc)[MI][NI]) {
+                                              int64_t k_end, char *lds, Acc4 (&total)[MI][NI]) {
     const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / kWavesN * WM, wn = wave % kWavesN * WN;
     const uint32_t lds_at =
@@ -250,6 +259,21 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < MI; ++i) fa[i] = A::fragment(lds, wm + i * 16, 0);
     int buf = 0;
+    Acc4 own[kJoin ? MI : 1][kJoin ? NI : 1] = {};
+    Acc4(&acc)[MI][NI] = [&]() -> Acc4(&)[MI][NI] {
+      if constexpr (kJoin > 0) return own;
+      else return total;
+    }();
+    auto join = [&] {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          total[i][j] += acc[i][j];
+          acc[i][j] = Acc4{0.f, 0.f, 0.f, 0.f};
+        }
+    };
+    int steps = 0;
     for (int64_t k = k_begin; k < k_end; k += kStep) {
       const int next = buf + 1 == STAGES ? 0 : buf + 1;
       const char *cur = lds + buf * kStage, *then = lds + next * kStage;
@@ -291,7 +315,13 @@ struct Tile {
         }
       }
       buf = next;  // (Loads beyond k_end are of zeros.)
+      if constexpr (kJoin > 0)
+        if (++steps == kJoin) {
+          join();
+          steps = 0;
+        }
     }
+    if constexpr (kJoin > 0) join();
     __builtin_amdgcn_sched_barrier(0);
     wait_and_meet<0>();
   }

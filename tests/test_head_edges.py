@@ -308,6 +308,30 @@ def test_rows_of_the_weight_megabytes_apart(dtype):
     assert torch.equal(got.row_loss, linear_softmax_grad(h[:3], w, y[:3]).row_loss)
 
 
+# -- long sums ------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("rows,width,vocab", [(8, 65536, 140), (33, 16384, 300), (100, 8192, 260)])
+def test_long_sums_of_one_sign(rows, width, vocab, dtype):
+    """Sums of equal terms, whose roundings lean to one side: at most 256 terms
+    are added to one sum before it is added to the next, so that a score is off
+    by (256 + width / 128) e of its size, where one chain would take width / 4
+    steps (width / 32 in 16 bits); lse and losses as scores, and 640 e of lse."""
+    print(f"[case] head long sums {rows} x {width} x {vocab} {dtype}", flush=True)
+    t = DTYPES[dtype]
+    c = torch.linspace(1.0, 1.9, vocab).to(t).cuda()
+    w = (c * 20 / width).to(t)[:, None].expand(vocab, width).contiguous()
+    h = torch.full((rows, width), 1 / 3).to(t).cuda()
+    y = torch.arange(rows).cuda() * 7 % vocab
+    z = h[0, 0].double() * width * w[:, 0].double()
+    lse = torch.logsumexp(z, 0)
+    off = (256 + width / 128) * E * float(z.max())
+    for got in (linear_softmax_loss(h, w, y), linear_softmax_grad(h, w, y)):
+        assert float((got.lse.double() - lse).abs().max()) <= off + 640 * E * float(lse)
+        assert float((got.row_loss.double() - (lse - z[y])).abs().max()) \
+            <= 2 * off + 640 * E * float(lse)
+
+
 # -- the label's value ----------------------------------------------------------
 def label_share(got, exact, along, own):
     """Root mean square over rows of the relative error that all of a row's
