@@ -190,10 +190,22 @@ __global__ __launch_bounds__(1024) void k_head_prepare(const PrepareArgs a) {
 // kernels' own times, in one launch and in two: 3.4 and 6.6 us for 128 rows of 512,
 // 5.5 and 7.9 for 1,024, 9.9 and 10.1 for 2,048, 20 and 15 for 4,096.
 constexpr int kCountRows = 2048;
+
+// Few rows of 16 bits with gradient stand twice among the packed rows, the second
+// time from a row on that is told (0: once), and what rounding takes of d loss /
+// d score stands beside the second ones: d_weight then sums both, and its operand
+// has twice the digits.  A label's rounding would be most of its class's error
+// otherwise: d_weight's was 1.6 times that of the rounded result at 1, 2 and 11
+// rows, and is 1.0 to 1.05; beyond kTwiceRows, where labels' errors average, it is
+// 1.1 to 1.4.  Kernel times with and without: 112 and 110 us (16 x 2,048 x 32,000
+// bf16), 950 and 880 (64 x 4,096 x 131,072); 1,200 and 1,080 at 100 rows.
+constexpr int kTwiceRows = 64;
+static_assert(2 * kTwiceRows <= kRowPad && kTwiceRows % 32 == 0, "both fit what is packed anyway");
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack_hidden(const T *hidden, int64_t stride,
                                                      int32_t width, int32_t wide,
-                                                     const PrepareArgs a, T *packed, T *d_hidden,
+                                                     const PrepareArgs a, T *packed,
+                                                     int32_t again, T *d_hidden,
                                                      int64_t d_stride) {
   __shared__ double tmp[256];
   const int32_t b = (int32_t)blockIdx.x, rows = a.rows;
@@ -212,13 +224,17 @@ __global__ __launch_bounds__(256) void k_pack_hidden(const T *hidden, int64_t st
     const int32_t n = p;
     p += b - rows;
     if (p >= (n + kRowPad - 1) / kRowPad * kRowPad) return;
+    if (again && p >= again && p < again + n) return;
     for (int32_t d = (int32_t)threadIdx.x; d < wide; d += 256) packed[(int64_t)p * wide + d] = (T)0.f;
     return;
   }
   if (p >= 0) {
     const T *from = hidden + (int64_t)b * stride;
-    for (int32_t d = (int32_t)threadIdx.x; d < wide; d += 256)
-      packed[(int64_t)p * wide + d] = d < width ? from[d] : (T)0.f;
+    for (int32_t d = (int32_t)threadIdx.x; d < wide; d += 256) {
+      const T x = d < width ? from[d] : (T)0.f;
+      packed[(int64_t)p * wide + d] = x;
+      if (again) packed[(int64_t)(again + p) * wide + d] = x;
+    }
   } else if (d_hidden) {
     for (int32_t d = (int32_t)threadIdx.x; d < width; d += 256)
       d_hidden[(int64_t)b * d_stride + d] = (T)0.f;
@@ -521,8 +537,8 @@ template <typename T>
 __global__ __launch_bounds__(kRowThreads) void k_rows(
     HeadInfo *info, int32_t piece, int32_t pieces, const int32_t *idx, const int32_t *lab,
     const float *u, float softcap, float z_loss, float grad_scale, int32_t tiles, int32_t tile_v,
-    const float2 *stats, const float *z_label, T *P, int64_t ldp, float *own_rest,
-    float *row_loss, float *lse_out) {
+    const float2 *stats, const float *z_label, T *P, int64_t ldp, int32_t again,
+    float *own_rest, float *row_loss, float *lse_out) {
   __shared__ float red[2 * kRowThreads / 64];
   constexpr int kVec = 16 / (int)sizeof(T), kVecs = 4;
   const Piece pc = piece_of(info->rows, piece, pieces);
@@ -532,6 +548,7 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
   const int32_t n = (int32_t)(ldp / kVec);
   if (r >= pc.rows) {
     // The products read whole steps of rows: zeros behind the last one.
+    if (again && r >= again && r < again + pc.rows) return;
     if (P && r < (pc.rows + kRowPad - 1) / kRowPad * kRowPad)
       for (int32_t i = tid; i < n; i += kRowThreads) row[i] = Int4{0, 0, 0, 0};
     return;
@@ -559,6 +576,7 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
   // k_d_hidden_sum adds it times the label's row of the weight.
   if (tid == 0) own_rest[r] = own - (float)(T)own;
   const float scale = g * (1.f + zl) / (kExpScale<T> * sum.y);
+  Int4 *rest = again ? row + (int64_t)again * n : nullptr;
   const int tile_shift = 31 - __clz(tile_v / kVec);
   for (int32_t i0 = tid; i0 < n; i0 += kRowThreads * kVecs) {
     Int4 x[kVecs];
@@ -577,11 +595,15 @@ __global__ __launch_bounds__(kRowThreads) void k_rows(
       if (i >= n) continue;
       const float by = expf(f[k] - sum.x) * scale;
       typedef T TV __attribute__((ext_vector_type(kVec)));
-      TV v = __builtin_bit_cast(TV, x[k]);
+      TV v = __builtin_bit_cast(TV, x[k]), low;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        v[e] = (T)(i * kVec + e == y ? own : (float)v[e] * by);
+      for (int e = 0; e < kVec; ++e) {
+        const float d = i * kVec + e == y ? own : (float)v[e] * by;
+        v[e] = (T)d;
+        low[e] = (T)(d - (float)v[e]);
+      }
       row[i] = __builtin_bit_cast(Int4, v);
+      if (rest) rest[i] = __builtin_bit_cast(Int4, low);
     }
   }
 }
@@ -604,7 +626,7 @@ struct ProductArgs {
   float *sum;
   void *d_weight;
   int64_t dw_stride;
-  int32_t dw_vec;
+  int32_t dw_vec, again;
 };
 
 // d_hidden of a piece: BM columns x BN rows over a part of the vocabulary, as
@@ -662,7 +684,8 @@ __device__ __forceinline__ void d_weight_tile(const ProductArgs &g, uint32_t blo
   a.init(static_cast<const T *>(g.packed) + (int64_t)pc.begin * wide, wide, d0, wide);
   b.init(static_cast<const T *>(g.P), g.ldp, v0, (int32_t)g.ldp);
   Acc4 acc[TL::MI][TL::NI] = {};
-  TL::walk(a, b, 0, (pc.rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
+  const int32_t rows = pc.rows ? g.again + pc.rows : 0;
+  TL::walk(a, b, 0, (rows + TL::kStep - 1) / TL::kStep * TL::kStep, lds, acc);
   const float lift = g.info->lift;
   if (pieces > 1) {
     const int wave = (int)threadIdx.x >> 6, l = (int)threadIdx.x & 63;
@@ -1031,9 +1054,11 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
                          sizeof(T) == 4, std::is_same<T, _Float16>::value, idx, lab, u, pos,
                          c.row_loss, c.lse, info};
   const bool count = p.rows <= kCountRows;
+  const int32_t again =
+      c.grad && sizeof(T) == 2 && p.rows <= kTwiceRows ? (int32_t)round_up(p.rows, 32) : 0;
   if (!count) k_head_prepare<<<1, 1024, 0, st>>>(prep);
   k_pack_hidden<T><<<(unsigned)p.rows + kRowPad + (count ? 1 : 0), 256, 0, st>>>(
-      static_cast<const T *>(c.hidden), c.h_stride, p.width, p.wide, prep, packed,
+      static_cast<const T *>(c.hidden), c.h_stride, p.width, p.wide, prep, packed, again,
       static_cast<T *>(c.d_hidden), c.dh_stride);
   const LossArgs loss{info, idx, u, c.row_loss, c.loss};
   const int64_t piece = std::min<int64_t>(p.rows, p.piece_rows);
@@ -1054,11 +1079,11 @@ int run_head(hipStream_t st, const HeadPlan &p, const HeadCall &c) {
         k_range<<<kRangeBlocks, 1024, 0, st>>>(info, k, p.pieces, p.tiles, stats);
     k_rows<T><<<(unsigned)(c.grad ? p.piece_rows : piece), kRowThreads, 0, st>>>(
         info, k, p.pieces, idx, lab, u, c.softcap, c.z_loss, c.grad_scale, p.tiles, p.tile_v, stats,
-        z_label, P, p.ldp, own_rest, c.row_loss, c.lse);
+        z_label, P, p.ldp, again, own_rest, c.row_loss, c.lse);
     if (!c.grad) continue;
     const ProductArgs g{P, p.ldp, packed, p.wide, p.vocab, p.width, info, k, p.pieces, weight,
                         w_stride, w_width, p.splits, p.split_v, part, part_stride, sum, c.d_weight,
-                        c.dw_stride, dw_vec};
+                        c.dw_stride, dw_vec, again};
     const unsigned hidden = (unsigned)(tiles_of(p.d_hidden, w_width, piece) * p.splits);
     const unsigned weights = (unsigned)tiles_of(p.d_weight, p.width, p.vocab);
     bool both = false;

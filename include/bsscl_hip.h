@@ -512,10 +512,11 @@ int bsscl_engine_stats(bsscl_engine *eng, double *out, int32_t cap,
  * Sums run in float32.  d loss / d score is rounded to the inputs' dtype as
  * operand of the two products, divided by the largest row weight first (so that
  * equal weights are exact); what that takes of the label's value is added to
- * d_hidden again.  In float16 it holds at least 2^-35 of the largest row
- * weight; where 1 + 2 zeta lse may exceed 32 in either sign, 2^-39 of that
- * weight times the largest such value (lse taken from the lowest maximum of 128
- * or 256 classes to the highest score plus log vocab).
+ * d_hidden again, and up to 64 rows what it takes of all values to d_weight.
+ * In float16 it holds at least 2^-35 of the largest row weight; where 1 + 2 zeta
+ * lse may exceed 32 in either sign, 2^-39 of that weight times the largest such
+ * value (lse taken from the lowest maximum of 128 or 256 classes to the highest
+ * score plus log vocab).
  * 1 <= rows <= 8000000, 1 <= width <= 65536, 1 <= vocab <= 4000000.
  */
 int bsscl_head_workspace(int32_t dtype, int64_t rows, int64_t width, int64_t vocab,

@@ -432,3 +432,30 @@ def test_a_missing_backward_is_said_on_the_gpu(rows):
     assert not any(t.requires_grad for t in got)
     h.backward(got.d_hidden)
     assert torch.equal(h.grad, got.d_hidden)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [1, 20, 32, 33, 64])
+def test_label_s_value_is_not_rounded_in_d_weight_of_few_rows(rows, dtype):
+    """Labels of any probability and unequal weights, rows left out among them.
+    The outputs' rounding leaves sqrt(3 / 4096) of 0.58 half steps in the share;
+    the label's own would be about 0.4 (of one row, anything below 1)."""
+    print(f"[case] head label's value in d_weight {rows} {dtype}", flush=True)
+    t = DTYPES[dtype]
+    width, vocab = 4096, 3001
+    g = torch.Generator().manual_seed(rows)
+    w = torch.randn(vocab, width, generator=g) / 32
+    y = torch.randperm(vocab, generator=g)[:rows]
+    h = torch.randn(rows, width, generator=g) + w[y] * (1 + 2 * torch.rand(rows, 1, generator=g))
+    h, w, y = h.to(t).cuda(), w.to(t).cuda(), y.cuda()
+    if rows > 5:
+        y[3:rows:7] = -1
+    u = (0.3 + 0.7 * torch.rand(rows, generator=g)).cuda()
+    m = Head(h, w, y, row_weight=u)
+    own = (torch.exp(-m.row_loss) - 1) * u.double() / u.double()[y >= 0].sum()
+    got = linear_softmax_grad(h, w, y, row_weight=u)
+    m.check(got)
+    k = y >= 0
+    assert label_share(got.d_weight[y[k]], m.d_weight[y[k]], m.h[k], own[k]) <= 0.1 * half_step(t)
+    assert label_share(got.d_hidden[k], m.d_hidden[k], m.w[y[k]], own[k]) <= 0.1 * half_step(t)
