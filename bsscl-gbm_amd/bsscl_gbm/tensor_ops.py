@@ -215,7 +215,7 @@ def _dense(t):
 
 def _list(torch, tensors, what):
     """(addresses, lengths, dtype codes, GPU) of the tensors as arrays for the
-    C ABI.  Lists are long and the kernels short: one pass of the tensors'
+    C ABI, and whether all are contiguous.  Lists are long and the kernels short: one pass of the tensors'
     methods each, and no loop of Python statements unless something is odd."""
     if not tensors:
         raise ValueError(f"{what} is empty")
@@ -246,21 +246,24 @@ def _list(torch, tensors, what):
         codes = array("i", [_dtype_codes[dtypes[0]]]) * len(tensors)
     else:
         codes = array("i", map(_dtype_codes.__getitem__, dtypes))
-    return ptrs, lengths, codes, devices.pop()
+    return ptrs, lengths, codes, devices.pop(), dense
 
 
 def _norm(tensors, inv_scale, max_norm, out):
     torch = _torch()
     tensors = list(tensors)
-    ptrs, lengths, codes, index = _list(torch, tensors, "tensors")
+    ptrs, lengths, codes, index, dense = _list(torch, tensors, "tensors")
     n = len(tensors)
     outs = ptrs
     if out is not None:
         out = list(out)
-        outs, _, out_codes, out_index = _list(torch, out, "out")
-        if len(out) != n or out_codes != codes or out_index != index or any(
-                o.shape != t.shape or o.stride() != t.stride() or o.is_neg() != t.is_neg()
-                for o, t in zip(out, tensors)):
+        outs, _, out_codes, out_index, out_dense = _list(torch, out, "out")
+        Tensor = torch.Tensor
+        if (len(out) != n or out_codes != codes or out_index != index
+                or not all(map(Tensor.is_same_size, out, tensors))
+                or not (dense and out_dense)  # (contiguous values lie alike)
+                and any(o.stride() != t.stride() for o, t in zip(out, tensors))
+                or list(map(Tensor.is_neg, out)) != list(map(Tensor.is_neg, tensors))):
             raise ValueError("out must match tensors in number, shape, strides, dtype and GPU")
 
     def at(a):

@@ -293,3 +293,19 @@ def test_tensors_saved_for_backward_are_known_to_be_written():
     assert float(t[0]) == pytest.approx(0.1)
     clip_grads([t], 0.5)  # an inference tensor counts no versions
     assert float(t[0]) == pytest.approx(0.05)
+
+
+@pytest.mark.gpu
+def test_out_of_the_same_memory_order():
+    """Strides of axes of size 1 say nothing; others, shapes and negated views
+    have to match."""
+    x = torch.randn(1, 64, generator=torch.Generator().manual_seed(3)).cuda()
+    t = torch.as_strided(x, (1, 64), (7, 1))
+    o = torch.empty(1, 64, device="cuda")
+    check([t], [o], clip_grads([t], 0.5, out=[o]), 0.5, 1.0)
+    a, b = torch.ones(8, 16, device="cuda"), torch.ones(16, 8, device="cuda")
+    for ts, out in (([a], [b]), ([a], [b.t()]), ([b.t()], [a]), ([a, b], [a.clone(), b.t()]),
+                    ([a], [torch._neg_view(a.clone())]), ([a], [a.clone(), b])):
+        with pytest.raises(ValueError, match="out must match"):
+            clip_grads(ts, 1.0, out=out)
+    clip_grads([b.t()], 1.0, out=[torch.empty_like(b).t()])
