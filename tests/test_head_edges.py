@@ -219,6 +219,19 @@ def test_few_rows_that_weigh_nothing(rows):
         assert all(not t.any() for t in got)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("rows", [1, 20, 64])
+def test_few_rows_all_left_out(rows, dtype):
+    """No row counts: zeros, whatever the rows hold."""
+    print(f"[case] head few rows left out {rows} {dtype}", flush=True)
+    h, w, y = make(rows, 64, 9000, DTYPES[dtype], seed=rows)
+    h[:], y[:] = float("nan"), -100
+    for r in (linear_softmax_grad(h, w, y), linear_softmax_grad(h, w, y, reduction="sum"),
+              linear_softmax_loss(h, w, y)):
+        assert all(not t.any() for t in r)
+
+
 # -- the ends of the sizes ------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
