@@ -273,7 +273,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 // Classes are the m of the tile, so that a lane holds 4 MI classes of each of
 // its rows and a row's maximum and sum take two lane exchanges and, where two
 // waves share it, one through LDS.  With many rows the matrix cores are the
-// bound (6,144 x 4,096 x 131,072 bf16 5.3 ms, 1.25 PFLOP/s with 1.6 GB of
+// bound (6,144 x 4,096 x 131,072 bf16 5.3 to 5.5 ms, 1.2 PFLOP/s with 1.6 GB of
 // exponentials written).  A tile's start and end cost 10 us, with a cap 19, and
 // writing the exponentials 1 to 16 more (1,536 rows x 32,768 classes bf16, three
 // rounds of tiles: 22, 33, 60 and 122 us a round at widths 512 to 4,096, with
@@ -733,8 +733,8 @@ __global__ __launch_bounds__(TL::kThreads) void k_d_weight(const ProductArgs g) 
 }
 // Both in one launch, d_hidden's long tiles (`hidden` blocks, a multiple of 8)
 // first: d_weight's short ones fill the CUs that they leave (1,500 x 2,048 x
-// 32,003 fp16 422 us, 501 in two launches; 6,144 x 4,096 x 131,072 bf16 10.2 ms,
-// 1.3 PFLOP/s, the same in two).
+// 32,003 fp16 422 us, 501 in two launches; 6,144 x 4,096 x 131,072 bf16 10.1 to
+// 10.5 ms, 1.3 PFLOP/s, the same in two).
 template <typename TH, typename TW>
 __global__ __launch_bounds__(TH::kThreads) void k_products(const ProductArgs g, uint32_t hidden) {
   static_assert(TH::kThreads == TW::kThreads);
