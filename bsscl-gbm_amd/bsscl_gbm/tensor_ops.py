@@ -215,8 +215,9 @@ def _dense(t):
 
 def _list(torch, tensors, what):
     """(addresses, lengths, dtype codes, GPU) of the tensors as arrays for the
-    C ABI, and whether all are contiguous.  Lists are long and the kernels short: one pass of the tensors'
-    methods each, and no loop of Python statements unless something is odd."""
+    C ABI, and whether all are contiguous.  Lists are long and the kernels short:
+    one pass of the tensors' methods each, and no loop of Python statements unless
+    something is odd."""
     if not tensors:
         raise ValueError(f"{what} is empty")
     Tensor = torch.Tensor
