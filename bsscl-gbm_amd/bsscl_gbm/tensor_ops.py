@@ -180,7 +180,8 @@ def linear_softmax_loss(hidden, weight, labels, *, row_weight=None, reduction="m
     linear_softmax_grad.
     """
     return SoftmaxLoss(*_without_graph(
-        _torch(), lambda: _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, None),
+        _torch(),
+        lambda: _head(hidden, weight, labels, row_weight, reduction, softcap, z_loss, None),
         (hidden, weight, row_weight)))
 
 
